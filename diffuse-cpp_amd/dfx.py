@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libdiffuse.so")
 
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K = 0, 1, 8, 12, 14, 15
+TYPE_F8 = 101                               # E4M3 cells of a paged cache
 SCHED_COSINE, SCHED_LINEAR = 0, 1
 LOW_CONFIDENCE, RANDOM, ENTROPY_EXIT, MASKGIT_PLUS, TOPK_MARGIN = 0, 1, 2, 3, 4
 ATTN_SPLIT_BF16, ATTN_EXACT = 0, 1          # dfx_attention_ex modes (include/dfx.h)
@@ -80,6 +81,18 @@ class SynthSpec(C.Structure):
                 ("n_threads", C.c_int32)]
 
 
+class PagedCache(C.Structure):
+    """dfx_paged_cache (include/dfx.h): the pages of keys and values of many sequences."""
+    _fields_ = [("type", C.c_int32), ("page_size", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32),
+                ("n_pages", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("scale", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    """dfx_paged_batch (include/dfx.h): rows, key counts and page ids of the sequences, on the device."""
+    _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("rows", C.c_void_p), ("n_keys", C.c_void_p),
+                ("pages", C.c_void_p), ("ld_pages", C.c_int64), ("max_keys", C.c_int64)]
+
+
 ROW_STAT = np.dtype([("token", "<i4"), ("best", "<f4"), ("second", "<f4"), ("entropy", "<f4")])
 CANDIDATE = np.dtype([("pos", "<i4"), ("token", "<i4"), ("confidence", "<f4"), ("entropy", "<f4")])
 
@@ -142,6 +155,11 @@ def _declare(L):
         "dfx_select": (I32, [P, I32, I32, F, I32, P, P, P]),
         "dfx_select_from_stats": (I32, [P, P, I32, I32, F, I32, P, P, P, P]),
         "dfx_make_candidates": (I32, [P, P, I32, I32, P, P]),
+        "dfx_paged_append": (I32, [P, P, P, I32, P, I64, I32, P, P]),
+        "dfx_paged_attention_ws_bytes": (S, [P, P, I32, I32]),
+        "dfx_paged_attention": (I32, [P, P, P, I32, I32, I32, I32, P, P, P]),
+        "dfx_token_logprobs_ws_bytes": (S, [I64, I64, I32]),
+        "dfx_token_logprobs": (I32, [P, I64, I64, P, I64, I64, P, I32, P, P, I32, P, P, P, P]),
         "dfx_quantize_rows": (I32, [I32, P, I64, I64, P]),
         "dfx_quantize_file": (I32, [C.c_char_p, C.c_char_p, C.c_char_p, I32]),
         "dfx_synth_model": (I32, [C.c_char_p, C.POINTER(SynthSpec)]),

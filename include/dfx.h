@@ -9,7 +9,7 @@
  * named *_alloc / *_new / *_load.
  *
  * Two levels:
- *   1. Kernel entry points (dfx_dequant ... dfx_select): one HIP kernel (or a
+ *   1. Kernel entry points (dfx_dequant ... dfx_token_logprobs): one HIP kernel (or a
  *      fixed short sequence) on caller-owned device buffers.  Each replaces a
  *      GGML CPU op of the reference graph, cited per function.
  *   2. Model / context entry points (dfx_model_load ... dfx_generate): the
@@ -42,6 +42,7 @@ enum {
     DFX_TYPE_Q4_K = 12,
     DFX_TYPE_Q6_K = 14,
     DFX_TYPE_Q8_K = 15,
+    DFX_TYPE_F8   = 101,   /* OCP E4M3 (no GGML type): cells of a paged cache only */
 };
 
 const char * dfx_last_error(void);
@@ -306,6 +307,95 @@ int dfx_ar_greedy(float * row, int64_t V, int32_t * state, int repeat_last_n, fl
  * over i of (x[m][i] - x_in[m][i])^2 with the difference and square in float and the
  * sum in double in increasing i.  x, x_in: device [M][d]; out: device double [M]. */
 int dfx_layer_impact(const float * x, const float * x_in, int64_t M, int64_t d, double * out, void * stream);
+
+/* ---- many sequences: a paged key / value cache ----
+ * No counterpart in the reference (one sequence per context): for callers that serve or score
+ * several sequences in one pass.
+ *
+ * A cache is n_pages pages of page_size tokens (16, 32, 64, 128 or 256), each divided into blocks
+ * of 16 tokens.  Cells are DFX_TYPE_F16, or DFX_TYPE_F8 with one power of two per block, KV head
+ * and side (2^k, k in -15..7, so that a cell times its scale is an f16 value exactly):
+ *   k      [n_pages][Hkv][page_size][hd]             cells
+ *   v      [n_pages][Hkv][page_size / 16][hd][16]    cells, a block's tokens innermost
+ *   scale  [n_pages][Hkv][page_size / 16][2]         f32, of k then of v (DFX_TYPE_F8 only)
+ * k, v start at 16-byte boundaries, scale at an 8-byte one; hd 64 or 128.
+ *
+ * A batch names the rows and the pages of n_seqs sequences, all in device memory, so that a
+ * captured call follows what the caller writes there: sequence s has the rows rows[s] ..
+ * rows[s + 1] - 1 (none where they are equal) of the n_rows rows that the row matrices hold, and
+ * they stand at the LAST positions of its n_keys[s] keys.  The key at position p is in page
+ * pages[s * ld_pages + p / page_size].  Rows at or behind rows[n_seqs] belong to no sequence and
+ * their outputs are left as they were.  max_keys bounds n_keys on the host: it sizes the workspace
+ * and the split of long caches over the chip (a sequence with more keys is computed all the same).
+ * What is out of range is bounded on the device: n_keys is held in 0 .. ld_pages * page_size,
+ * rows in 0 .. n_rows, and a page id outside 0 .. n_pages - 1 is no page (its keys are neither
+ * written nor seen). */
+typedef struct {
+    int32_t type;                /* DFX_TYPE_F16 or DFX_TYPE_F8 */
+    int32_t page_size;
+    int32_t n_head_kv, head_dim;
+    int64_t n_pages;
+    void  * k;
+    void  * v;
+    float * scale;               /* NULL with DFX_TYPE_F16 */
+} dfx_paged_cache;
+
+typedef struct {
+    int32_t n_seqs;
+    int32_t n_rows;
+    const int32_t * rows;        /* device [n_seqs + 1], not decreasing */
+    const int32_t * n_keys;      /* device [n_seqs] */
+    const int32_t * pages;       /* device [n_seqs][ld_pages] */
+    int64_t ld_pages;
+    int64_t max_keys;
+} dfx_paged_batch;
+
+/* NEOX RoPE of the rows' Q and K (as dfx_rope_store, bit for bit in f32) and the append of K and V
+ * to the cache, in one launch.  qkv: [n_rows][(H + 2 Hkv) hd] f32 (Q | K | V); tab:
+ * [n_pos][hd/2][cos, sin] f32; q_out: [n_rows][H][hd] of q_type (DFX_TYPE_F16 or DFX_TYPE_F32).
+ * DFX_TYPE_F8: a block whose first token is written takes the least power of two with which its
+ * new finite values stay within E4M3's +-448; a block that keeps earlier tokens takes the larger
+ * of that and its own, and the kept cells are brought to it (exact but for cells that fall below
+ * E4M3's normal range).  Values beyond the largest scale saturate; infinities and NaN become NaN.
+ * Writing the same positions again (a step over a block of positions that is recomputed) starts
+ * with the tokens before them.  A row whose position is negative or not below n_pos is skipped.
+ * Two sequences must not write to one page; pages that a sequence only reads may be shared.
+ * qkv, tab and q_out start at 16-byte boundaries. */
+int dfx_paged_append(const dfx_paged_cache * cache, const dfx_paged_batch * batch, const float * qkv, int n_head,
+                     const float * tab, int64_t n_pos, int q_type, void * q_out, void * stream);
+
+/* Attention of the batch's rows over their sequences' cached keys (their own included, appended
+ * before): out[r][h][:] = sum_j softmax_j(q_rh . k_j / sqrt(hd)) v_j, query head h reading KV head
+ * h / (H / Hkv).  A row at position p sees the keys 0 .. n_keys - 1, or with causal != 0 those up
+ * to p, of them with window > 0 (causal only) the last `window`.  A row that sees no key gives
+ * zeros; keys that a row does not see never reach it, whatever they hold (NaN included).
+ * q, out: [n_rows][H][hd] of `type`, 16-byte aligned: DFX_TYPE_F16 (products of f16 values,
+ * f32 sums, probabilities rounded to f16 before P V) or DFX_TYPE_F32 (q and the probabilities
+ * split into two f16 terms each: f32 accuracy on the f16 matrix cores).  An f16 `out` is the
+ * activation buffer of a dfx_gemm on F16 weights.
+ * ws: dfx_paged_attention_ws_bytes bytes (16-byte aligned; may be 0), or NULL: long caches are then
+ * not split over workgroups.  Calls sharing ws must not overlap.  The result does not depend on
+ * timing; it may depend on n_seqs, n_rows and max_keys, which choose the split. */
+size_t dfx_paged_attention_ws_bytes(const dfx_paged_cache * cache, const dfx_paged_batch * batch, int n_head, int type);
+int dfx_paged_attention(const dfx_paged_cache * cache, const dfx_paged_batch * batch, const void * q, int type,
+                        int n_head, int causal, int window, void * out, void * ws, void * stream);
+
+/* Log probabilities of given tokens, entropy and the best alternatives of logits rows, in one read
+ * of each row (the statistics of dfx_row_stats for scoring; src/diffuse-sampler.cpp:34-57 is the
+ * entropy).  Row i is logits row rows[i] (rows NULL: row i) of the [n_logits][ld] f32 matrix:
+ *   logprob[i][j]     = x_t - log sum exp x of the token t = tokens[i][j], j < n_tok (NaN for a
+ *                       token outside 0 .. V-1)
+ *   entropy[i]        = -sum p log p, in nats (NULL: not written)
+ *   top_id[i][j], top_logprob[i][j], j < n_top <= 64: the largest logits in falling order, the lowest
+ *                       index first among equal ones; NaN ranks as -inf; -1 and -inf beyond V
+ * A logits row outside 0 .. n_logits-1, and a row with NaN, +inf or nothing above -inf, has NaN for
+ * its probabilities and entropy (the former -1 for its ids).  n_tok, n_top may be 0 (their arrays
+ * are then not touched).  ws: dfx_token_logprobs_ws_bytes bytes, 16-byte aligned; calls sharing it
+ * must not overlap. */
+size_t dfx_token_logprobs_ws_bytes(int64_t n_rows, int64_t V, int n_top);
+int dfx_token_logprobs(const float * logits, int64_t ld, int64_t n_logits, const int32_t * rows, int64_t n_rows,
+                       int64_t V, const int32_t * tokens, int n_tok, float * logprob, float * entropy, int n_top,
+                       int32_t * top_id, float * top_logprob, void * ws, void * stream);
 
 /* ---- weight encoding, quantizer and synthetic models (host side) ---- */
 
