@@ -34,7 +34,7 @@ __device__ __forceinline__ int wave_find_seq(const paged_t & p, int m) {
 
 struct row_place { int s, pos, r0, r1; };   // s < 0: the row belongs to no sequence
 
-// Lane j < N (N = 1 or 16) gets the place of row m0 + j; the lanes above repeat them.  Decoding
+// Lane j < N (N a power of two) gets the place of row m0 + j; the lanes above repeat them.  Decoding
 // batches have a sequence per row, prompts one for all rows.
 template <int N> __device__ __forceinline__ row_place wave_places(const paged_t & p, int m0) {
     const int lane = threadIdx.x & 63;
@@ -108,34 +108,50 @@ __device__ __forceinline__ f8_choice f8_choose(float amax, bool kept, float old)
 // Append
 // ---------------------------------------------------------------------------
 // Waves: first the cells, one wave per (RT rows, KV head, side), each taking the blocks whose first
-// row of the call is among its RT rows; then Q, one wave per (16 rows, head).  RT = 1 where the rows
+// row of the call is among its RT rows; then Q, one wave per (rows of one pass, QHEADS heads), whose
+// angles are read once.  RT = 1 where the rows
 // belong to many sequences (each row enters a block of its own, and one wave per row keeps its chain
 // of dependent loads - places, page, scale, kept cells - alone on it), 16 otherwise.
 #define APPEND_WAVES 4
+#define QHEADS 4
 
 // (cos, sin) and the two halves of four pairs of a row
 struct rope4 {
     float4 a, b, c01, c23;
-    __device__ __forceinline__ void load(const float * src, const float * cs, int half) {
+    __device__ __forceinline__ void load_x(const float * src, int half) {
         a = *(const float4 *)src;
         b = *(const float4 *)(src + half);
+    }
+    __device__ __forceinline__ void load_angles(const float * cs) {
         c01 = *(const float4 *)cs;
         c23 = *(const float4 *)(cs + 4);
     }
-    __device__ __forceinline__ void turn(float (&y0)[4], float (&y1)[4]) const {
+    __device__ __forceinline__ void load(const float * src, const float * cs, int half) {
+        load_x(src, half);
+        load_angles(cs);
+    }
+    // a, b = the rotated halves
+    __device__ __forceinline__ void turn() {
 #pragma clang fp contract(off)
-        const float x0[4] = {a.x, a.y, a.z, a.w}, x1[4] = {b.x, b.y, b.z, b.w};
-        const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            y0[k] = x0[k] * c[k] - x1[k] * s[k];
-            y1[k] = x0[k] * s[k] + x1[k] * c[k];
-        }
+        const float4 x = a, y = b;
+        a = make_float4(x.x * c01.x - y.x * c01.y, x.y * c01.z - y.y * c01.w, x.z * c23.x - y.z * c23.y,
+                        x.w * c23.z - y.w * c23.w);
+        b = make_float4(x.x * c01.y + y.x * c01.x, x.y * c01.w + y.y * c01.z, x.z * c23.y + y.z * c23.x,
+                        x.w * c23.w + y.w * c23.z);
     }
 };
+__device__ __forceinline__ half4 to_half4(float4 x) {
+    return half4{(half_t)x.x, (half_t)x.y, (half_t)x.z, (half_t)x.w};
+}
+__device__ __forceinline__ float f8_max4(float m, float4 x) {
+    return fmaxf(m, fmaxf(fmaxf(f8_finite_abs(x.x), f8_finite_abs(x.y)), fmaxf(f8_finite_abs(x.z), f8_finite_abs(x.w))));
+}
+__device__ __forceinline__ uint32_t f8_cells4(float4 x, float inv) {
+    return f8_pack4(f8_ready(x.x, inv), f8_ready(x.y, inv), f8_ready(x.z, inv), f8_ready(x.w, inv));
+}
 
 template <int HD, bool F8, bool QF32>
-__global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, const float * __restrict__ qkv, int H,
+__global__ void __launch_bounds__(64 * APPEND_WAVES, 3) k_paged_append(paged_t p, const float * __restrict__ qkv, int H,
                                                                     const float * __restrict__ tab, int n_pos,
                                                                     void * __restrict__ q_out, int RT, int n_cell_waves,
                                                                     int n_waves) {
@@ -154,27 +170,32 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
     constexpr int RPP = 64 / LPR;                        // rows per pass of the wave
     const int lr = lane / LPR, j4 = 4 * (lane % LPR);
 
-    if (w >= n_cell_waves) {                             // ---- Q: 16 rows of one head
-        const int u = w - n_cell_waves, h = u % H, m0 = (u / H) * 16;
-        const row_place at = wave_places<16>(p, m0);
+    if (w >= n_cell_waves) {                             // ---- Q: RPP rows of QHEADS heads
+        const int groups = (H + QHEADS - 1) / QHEADS;
+        const int u = w - n_cell_waves, h0 = (u % groups) * QHEADS, m0 = (u / groups) * RPP, m = m0 + lr;
+        rope4 x[QHEADS];
+        const float * src = qkv + min(m, p.n_rows - 1) * ld + (int64_t)h0 * HD + j4;    // clamped: not stored
 #pragma unroll
-        for (int pass = 0; pass < 16 / RPP; pass++) {
-            const int j = pass * RPP + lr, m = m0 + j;
-            const int s = __shfl(at.s, j, WAVE), pos = __shfl(at.pos, j, WAVE);
-            if (s < 0 || pos < 0 || pos >= n_pos) continue;
-            rope4 x;
-            x.load(qkv + m * ld + (int64_t)h * HD + j4, tab + ((int64_t)pos * HALF + j4) * 2, HALF);
-            float y0[4], y1[4];
-            x.turn(y0, y1);
-            const int64_t o = ((int64_t)m * H + h) * HD + j4;
+        for (int k = 0; k < QHEADS; k++) x[k].load_x(src + (int64_t)min(k, H - 1 - h0) * HD, HALF);
+        const row_place at = wave_places<RPP>(p, m0);
+        const int s = __shfl(at.s, lr, WAVE), pos = __shfl(at.pos, lr, WAVE);
+        if (s < 0 || pos < 0 || pos >= n_pos) return;
+        x[0].load_angles(tab + ((int64_t)pos * HALF + j4) * 2);
+#pragma unroll
+        for (int k = 0; k < QHEADS; k++) {
+            if (h0 + k >= H) break;
+            x[k].c01 = x[0].c01;
+            x[k].c23 = x[0].c23;
+            x[k].turn();
+            const int64_t o = ((int64_t)m * H + h0 + k) * HD + j4;
             if constexpr (QF32) {
                 float * dst = (float *)q_out + o;
-                *(float4 *)dst = make_float4(y0[0], y0[1], y0[2], y0[3]);
-                *(float4 *)(dst + HALF) = make_float4(y1[0], y1[1], y1[2], y1[3]);
+                *(float4 *)dst = x[k].a;
+                *(float4 *)(dst + HALF) = x[k].b;
             } else {
                 half_t * dst = (half_t *)q_out + o;
-                *(half4 *)dst = half4{(half_t)y0[0], (half_t)y0[1], (half_t)y0[2], (half_t)y0[3]};
-                *(half4 *)(dst + HALF) = half4{(half_t)y1[0], (half_t)y1[1], (half_t)y1[2], (half_t)y1[3]};
+                *(half4 *)dst = to_half4(x[k].a);
+                *(half4 *)(dst + HALF) = to_half4(x[k].b);
             }
         }
         return;
@@ -182,6 +203,9 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
 
     // ---- cells: RT rows of one head and side
     const int unit = w % (2 * Hkv), kvh = unit >> 1, side = unit & 1, m0 = (w / (2 * Hkv)) * RT;
+    // one row: its line is on its way while its place is looked up
+    float warm = 0.0f;
+    if (RT == 1 && lane < HD / 16) warm = qkv[m0 * ld + (int64_t)(H + side * Hkv + kvh) * HD + 16 * lane];
     const row_place at = RT == 1 ? wave_places<1>(p, m0) : wave_places<16>(p, m0);
     const bool enters = lane < RT && at.s >= 0 && at.pos >= 0 && at.pos < limit &&
                         ((at.pos & 15) == 0 || m0 + lane == at.r0);
@@ -192,12 +216,12 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
         const int cnt = min(min(r1 - m, 16 - t0), limit - pos);             // new tokens t0 .. t0 + cnt - 1
         const int64_t blk = pg_block(p, s, kvh, pos);
         if (blk < 0) continue;
+        asm volatile("" : : "v"(warm));
         float old = 0.0f;
         if constexpr (F8) old = p.scale[2 * blk + side];
         if (side == 0) {
             // keys: rotated, cells [16][HD]
             constexpr int NP = 16 / RPP;
-            float y0[NP][4], y1[NP][4];
             float amax = 0.0f;
             const float * src = qkv + (int64_t)(H + kvh) * HD + j4;
             rope4 x[NP];
@@ -210,9 +234,8 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 if (i * RPP >= cnt) break;
-                x[i].turn(y0[i], y1[i]);
-#pragma unroll
-                for (int k = 0; k < 4; k++) amax = fmaxf(amax, fmaxf(f8_finite_abs(y0[i][k]), f8_finite_abs(y1[i][k])));
+                x[i].turn();
+                amax = f8_max4(f8_max4(amax, x[i].a), x[i].b);
             }
             if constexpr (F8) {
                 const f8_choice c = f8_choose(wave_max(amax), t0 > 0, old);
@@ -230,10 +253,8 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
                     const int r = i * RPP + lr;
                     if (r >= cnt) break;
                     uint8_t * dst = cell + (t0 + r) * HD + j4;
-                    *(uint32_t *)dst = f8_pack4(f8_ready(y0[i][0], inv), f8_ready(y0[i][1], inv),
-                                                f8_ready(y0[i][2], inv), f8_ready(y0[i][3], inv));
-                    *(uint32_t *)(dst + HALF) = f8_pack4(f8_ready(y1[i][0], inv), f8_ready(y1[i][1], inv),
-                                                         f8_ready(y1[i][2], inv), f8_ready(y1[i][3], inv));
+                    *(uint32_t *)dst = f8_cells4(x[i].a, inv);
+                    *(uint32_t *)(dst + HALF) = f8_cells4(x[i].b, inv);
                 }
                 if (lane == 0) p.scale[2 * blk] = c.scale;
             } else {
@@ -243,8 +264,8 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
                     const int r = i * RPP + lr;
                     if (r >= cnt) break;
                     half_t * dst = cell + (t0 + r) * HD + j4;
-                    *(half4 *)dst = half4{(half_t)y0[i][0], (half_t)y0[i][1], (half_t)y0[i][2], (half_t)y0[i][3]};
-                    *(half4 *)(dst + HALF) = half4{(half_t)y1[i][0], (half_t)y1[i][1], (half_t)y1[i][2], (half_t)y1[i][3]};
+                    *(half4 *)dst = to_half4(x[i].a);
+                    *(half4 *)(dst + HALF) = to_half4(x[i].b);
                 }
             }
         } else {
@@ -262,12 +283,28 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 if (i * RV >= cnt) break;
-                amax = fmaxf(amax, fmaxf(fmaxf(f8_finite_abs(x[i].x), f8_finite_abs(x[i].y)),
-                                         fmaxf(f8_finite_abs(x[i].z), f8_finite_abs(x[i].w))));
+                amax = f8_max4(amax, x[i]);
             }
             f8_choice c = {1.0f, 1.0f};
             if constexpr (F8) c = f8_choose(wave_max(amax), t0 > 0, old);
             const float inv = 1.0f / c.scale;
+            if (cnt == 1 && c.ratio == 1.0f) {
+                // one token, the kept ones as they are: its cells alone are written, none read
+                if (vr == 0) {
+                    uint8_t * cell = (uint8_t *)p.v + (blk * (16 * HD) + d4 * 16 + t0) * CELL;
+                    const float e[4] = {x[0].x, x[0].y, x[0].z, x[0].w};
+                    if constexpr (F8) {
+                        const uint32_t q = f8_cells4(x[0], inv);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) cell[16 * k] = (uint8_t)(q >> (8 * k));
+                        if (lane == 0) p.scale[2 * blk + 1] = c.scale;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) ((uint16_t *)cell)[16 * k] = f2h(e[k]);
+                    }
+                }
+                continue;
+            }
             uint8_t * vt = vt_all[wv];
 #pragma unroll
             for (int i = 0; i < NP; i++) {
@@ -275,8 +312,7 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) k_paged_append(paged_t p, c
                 if (r >= cnt) break;
                 const float e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                 if constexpr (F8) {
-                    const uint32_t q = f8_pack4(f8_ready(e[0], inv), f8_ready(e[1], inv), f8_ready(e[2], inv),
-                                                f8_ready(e[3], inv));
+                    const uint32_t q = f8_cells4(x[i], inv);
 #pragma unroll
                     for (int k = 0; k < 4; k++) vt[(d4 + k) * 16 + t0 + r] = (uint8_t)(q >> (8 * k));
                 } else {
@@ -394,7 +430,8 @@ extern "C" int dfx_paged_append(const dfx_paged_cache * cache, const dfx_paged_b
     }
     const int RT = (int64_t)p.n_seqs * 8 > p.n_rows ? 1 : 16;
     const int64_t cell_waves = ((int64_t)(p.n_rows + RT - 1) / RT) * 2 * p.Hkv;
-    const int64_t waves = cell_waves + (int64_t)((p.n_rows + 15) / 16) * n_head;
+    const int q_rows = 64 / (cache->head_dim / 8);              // rows of a wave's pass
+    const int64_t waves = cell_waves + (int64_t)((p.n_rows + q_rows - 1) / q_rows) * ((n_head + QHEADS - 1) / QHEADS);
     const int np = (int)(n_pos < INT32_MAX ? n_pos : INT32_MAX);
     const dim3 grid((unsigned)((waves + APPEND_WAVES - 1) / APPEND_WAVES)), wg(64 * APPEND_WAVES);
 #define APPEND(HD, F8, QF32)                                                                                          \

@@ -16,6 +16,7 @@
 #include "dfx_pages.h"
 
 #include <algorithm>
+#include <atomic>
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -31,6 +32,9 @@ __device__ __forceinline__ half8 f8_half8(uint32_t w0, uint32_t w1, float scale)
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+__device__ __forceinline__ float16v mfma32(half8 a, half8 b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
 __device__ __forceinline__ float4v mfma16(half8 a, half8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -49,38 +53,57 @@ __device__ __forceinline__ float quad_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// maximum / sum over the two lanes l, l ^ 32
+__device__ __forceinline__ float half_max(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 // An f32 value as two f16 terms (the second rounded: 2^-23 of the value where it is f16-normal).
 __device__ __forceinline__ void split16(float x, half_t & hi, half_t & lo) {
     hi = (half_t)x;
     lo = (half_t)(x - (float)hi);
 }
 
+// Power of two by which an f32 query row is divided, so that its largest magnitude is in 2^8 .. 2^9
+// and the second terms keep their bits (rows of zeros and of no finite magnitude are left).
+__device__ __forceinline__ int q_exponent(float amax) {
+    if (!(amax > 0.0f && amax <= 3.402823466e38f)) return 0;
+    int ex;
+    (void)frexpf(amax, &ex);
+    return max(ex - 9, -100);
+}
+
 // NaN and infinities among the values.  A query that does not see a key has probability 0 for it, and
 // 0 times such a value is NaN; a probability that is 0 in f16, or the second term of a split one (0 or
-// negative), makes NaN of an infinite value that is seen.  So where a tile has such values and needs it
-// (NaN alone, seen by all, is right as it is), they are taken out (0 in their place), and a second
-// product of marks (NaN 2^14, -inf 2^7, +inf 1; a tile sums at most 64 of each) with visibility
-// (0 or 1) says what each output gets.
+// negative), makes NaN of an infinite value that is seen.  So they are taken out of the products (0 in
+// their place) and the key tiles that have them are noted, in a map of MAP_BITS tiles (tile modulo
+// that: a tile noted for another costs time, not a result); at the end the cells of those tiles are
+// looked through again, and what a query sees of them is added to its sums.
 //
-// Nonzero if one of the word's cells is NaN or infinite (exponent, in E4M3 all bits, of ones).
+// The word's cells that are NaN or infinite (exponent, in E4M3 all bits, of ones): their top bits.
 template <bool F8> __device__ __forceinline__ uint32_t special_bits(uint32_t w) {
     return F8 ? ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
-__device__ __forceinline__ void split_special(half8 v, half8 & fine, half8 & mark) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const uint16_t b = __builtin_bit_cast(uint16_t, (half_t)v[e]);
-        const bool sp = (b & 0x7c00u) == 0x7c00u;
-        fine[e] = sp ? (half_t)0.0f : (half_t)v[e];
-        mark[e] = !sp ? (half_t)0.0f : (b & 0x3ffu) ? (half_t)16384.0f : (b & 0x8000u) ? (half_t)128.0f : (half_t)1.0f;
+template <bool F8> __device__ __forceinline__ uint32_t without_special(uint32_t w) {
+    const uint32_t b = special_bits<F8>(w);
+    return w & ~(F8 ? (b >> 7) * 0xffu : (b >> 15) * 0xffffu);
+}
+#define MAP_BITS 512
+struct special_map {
+    uint32_t w[MAP_BITS / 32];
+    __device__ __forceinline__ void note(int t) { atomicOr(&w[(t & (MAP_BITS - 1)) >> 5], 1u << (t & 31)); }
+    __device__ __forceinline__ bool has(int t) const { return w[(t & (MAP_BITS - 1)) >> 5] >> (t & 31) & 1u; }
+    __device__ __forceinline__ bool any() const {
+        uint32_t a = 0;
+        for (int i = 0; i < MAP_BITS / 32; i++) a |= w[i];
+        return a != 0;
     }
-}
-__device__ __forceinline__ float special_of(float marks) {   // what is added to an output
-    if (marks == 0.0f) return 0.0f;
-    const int k = (int)marks;
-    const bool neg = (k & 16383) >= 128, pos = (k & 127) != 0;
-    return k >= 16384 || (neg && pos) ? __builtin_nanf("") : neg ? -INFINITY : INFINITY;
-}
+};
 
 // ---------------------------------------------------------------------------
 // Work: query tiles of ragged sequences
@@ -112,6 +135,66 @@ template <int T> __device__ __forceinline__ tile_at wave_tile(const paged_t & p,
     return {-1, 0, {0, 0, 0}};
 }
 
+// Sum over the wave, the same in every lane (and known to be: a scalar).
+__device__ __forceinline__ int wave_sum_i(int v) {
+    v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);        // within rows of 16 lanes
+    v += __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true);
+    return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
+           (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+
+template <int T> __device__ __forceinline__ tile_at one_tile(const paged_t & p, int G, int t) {
+    const seq_t q = pg_seq(p, 0);
+    return t < (q.n * G + T - 1) / T ? tile_at{0, t, q} : tile_at{-1, 0, {0, 0, 0}};
+}
+
+// The tiles of the batch in the order of their work, the ones with the most key tiles first (what runs
+// last is short, and neighbours are alike: workgroups go to the parts of the chip in turn).  The weight
+// k of tile t: the largest with more than t tiles of at least that weight, found bit by bit.  Up to 64
+// sequences (a lane each); more: sequence by sequence, each from its end.
+template <int T> __device__ __forceinline__ tile_at wave_tile_by_work(const paged_t & p, int G, int causal, int window, int t) {
+    const int lane = threadIdx.x & 63;
+    if (p.n_seqs > 64 || p.n_seqs == 1) {
+        tile_at at = p.n_seqs == 1 ? one_tile<T>(p, G, t) : wave_tile<T>(p, G, t);
+        if (at.s >= 0) at.tile = (at.q.n * G + T - 1) / T - 1 - at.tile;
+        return at;
+    }
+    seq_t q = {0, 0, 0};
+    if (lane < p.n_seqs) q = pg_seq(p, lane);
+    const int nq = q.n * G, cnt = (nq + T - 1) / T, p0 = q.keys - q.n;
+    const int heaviest = window > 0 ? (window + 63) / 64 + 1 : 1 << 26;
+    // the sequence's first tile of weight k or more: its last row sees position 64 (k - 1)
+    auto first_of = [&](int k) {
+        if (k <= 0) return 0;
+        if (k > heaviest) return cnt;
+        if (!causal) return 64 * (int64_t)(k - 1) < q.keys ? 0 : cnt;
+        const int64_t f = ((int64_t)64 * (k - 1) - p0) * G;
+        return f <= 0 ? 0 : f > nq - 1 ? cnt : (int)f / T;
+    };
+    const int most = cnt ? min(max(q.keys - 1, 0) / 64 + 1, heaviest) : 0;
+    int k = 0;
+    for (int bit = 1 << 25; bit > 0; bit >>= 1) {
+        const int c = k | bit;
+        if (!__any(most >= c)) continue;                           // no tile is that heavy
+        if (wave_sum_i(cnt - first_of(c)) > t) k = c;
+    }
+    const int above = wave_sum_i(cnt - first_of(k + 1));           // tiles heavier than k
+    const int from_k = first_of(k), mine = first_of(k + 1) - from_k;
+    int sum = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(sum, o, WAVE);
+        if (lane >= o) sum += v;
+    }
+    const uint64_t has = __ballot(above + sum > t);
+    if (!has) return {-1, 0, {0, 0, 0}};
+    const int from = __ffsll((unsigned long long)has) - 1;
+    return {from, __builtin_amdgcn_readlane(from_k, from) + t - above - __builtin_amdgcn_readlane(sum - mine, from),
+            {__builtin_amdgcn_readlane(q.r0, from), __builtin_amdgcn_readlane(q.n, from),
+             __builtin_amdgcn_readlane(q.keys, from)}};
+}
+
 // Workgroup number -> (KV head, tile of the batch).  Workgroups go round the 8 XCDs, so head kvh's
 // tiles are put on XCD kvh % 8 (with fewer heads, which divide 8, on 8 / Hkv XCDs each): an L2 holds the
 // keys of its heads only.  Other head counts: heads in turn.
@@ -128,13 +211,100 @@ static unsigned unit_grid(int Hkv, int tiles) {
     return (unsigned)Hkv * (unsigned)tiles;
 }
 
+// Sum of the NaN and infinite values of column `dim` that a query sees among the noted tiles.
+template <int HD, bool F8>
+__device__ __forceinline__ float special_sum(const paged_t & p, const special_map & map, int s, int kvh, int dim,
+                                                       int t0, int t1, seen_t see, int keys) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int t = t0; t < t1; t++) {
+        if (!map.has(t - t0)) continue;
+#pragma unroll 1
+        for (int b = 0; b < 4; b++) {
+            const int k0 = 64 * t + 16 * b;
+            const int lo = pg_clamp(see.lo - k0, 0, 16), hi = pg_clamp(min(see.hi + 1, keys) - k0, 0, 16);
+            if (hi <= lo) continue;
+            const int64_t blk = pg_block(p, s, kvh, k0);
+            if (blk < 0) continue;
+#pragma unroll 1
+            for (int j = lo; j < hi; j++) {
+                if constexpr (F8) {
+                    const uint8_t c = ((const uint8_t *)p.v)[(blk * HD + dim) * 16 + j];
+                    if ((c & 0x7f) == 0x7f) sum += __builtin_nanf("");
+                } else {
+                    const uint16_t c = ((const uint16_t *)p.v)[(blk * HD + dim) * 16 + j];
+                    if ((c & 0x7c00) == 0x7c00) sum += h2f(c);
+                }
+            }
+        }
+    }
+    return sum;
+}
+
 struct attn_t {
     const void * q;
     void * out;
     float * part_o;      // [parts][n_rows * H][hd] unscaled sums
     float * part_ml;     // [parts][n_rows * H][2] maximum, sum
+    int32_t * n_parts;   // [n_rows * H]
     int H, G, causal, window, chunk, parts, tiles;
 };
+
+// The four waves' maxima, sums and outputs ([4][T], [4][T], [4][T][HD + 4] in LDS) of a query tile as
+// one: results, or a part of them.
+template <int HD, bool F8, bool F32, int T>
+__device__ __forceinline__ void join_waves(const paged_t & p, const attn_t & a, const tile_at & at, const part_at & pt, int kvh,
+                                           int f0, int f1, const float * so, const float * sm, const float * sl,
+                                           const special_map & map) {
+    constexpr int OS = HD + 4;
+    const int keys = at.q.keys, p0 = keys - at.q.n;
+    const bool special = map.any();
+    for (int e = threadIdx.x; e < T * (HD / 4); e += 256) {
+        const int c = e / (HD / 4), d = 4 * (e % (HD / 4)), fc = f0 + c;
+        if (fc > f1) continue;
+        const float mx = fmaxf(fmaxf(sm[c], sm[T + c]), fmaxf(sm[2 * T + c], sm[3 * T + c]));
+        float sum = 0.0f;
+        float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float mw = sm[w * T + c], lw = sl[w * T + c];
+            const float r = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(mw - mx);
+            sum += r * lw;
+            const float4v x = *(const float4v *)(so + (w * T + c) * OS + d);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = fmaf(r, x[k], v[k]);
+        }
+        if (special)
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+                const float add = special_sum<HD, F8>(p, map, at.s, kvh, d + k, pt.t0, pt.t1,
+                                                      pg_seen(p0 + fc / a.G, keys, a.causal, a.window), keys);
+                v.x += k == 0 ? add : 0.0f;
+                v.y += k == 1 ? add : 0.0f;
+                v.z += k == 2 ? add : 0.0f;
+                v.w += k == 3 ? add : 0.0f;
+            }
+        const int64_t rh = (int64_t)(at.q.r0 + fc / a.G) * a.H + kvh * a.G + fc % a.G;
+        if (F32) v *= 1.0f / 16384.0f;
+        if (pt.parts == 1) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            v *= inv;
+            if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + d) = v;
+            else *(half4 *)((half_t *)a.out + rh * HD + d) = half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+        } else {
+            const int64_t at_part = (int64_t)blockIdx.y * p.n_rows * a.H + rh;
+            *(float4v *)(a.part_o + at_part * HD + d) = v;
+        }
+        if (d == 0 && a.parts > 1) {
+            const int64_t at_part = (int64_t)blockIdx.y * p.n_rows * a.H + rh;
+            if (blockIdx.y == 0) a.n_parts[rh] = pt.parts;
+            if (pt.parts > 1) {
+                a.part_ml[2 * at_part] = mx;
+                a.part_ml[2 * at_part + 1] = sum;
+            }
+        }
+    }
+}
 
 // ---------------------------------------------------------------------------
 // Few rows: 16 queries per workgroup, keys straight from memory
@@ -145,7 +315,7 @@ struct attn_t {
 // over the four tiles are the 16 tokens of block g.
 #define FEW_T 16
 template <int HD, bool F8, bool F32>
-__global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
+__global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 : 3) k_paged_few(paged_t p, attn_t a) {
     constexpr int KS = HD / 32;                 // 32-dim steps of S
     constexpr int DT = HD / 16;                 // 16-dim tiles of O
     constexpr int KW = F8 ? HD / 64 : HD / 32;  // 16-byte loads of a lane per S tile
@@ -153,10 +323,11 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
     constexpr int OS = HD + 4;                  // LDS floats per query
     __shared__ float so[4][FEW_T][OS];
     __shared__ float sm[4][FEW_T], sl[4][FEW_T];
+    __shared__ special_map map;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const unit_at un = unit_of(blockIdx.x, p.Hkv, a.tiles);
     if (un.kvh >= p.Hkv) return;
-    const tile_at at = wave_tile<FEW_T>(p, a.G, un.tile);
+    const tile_at at = wave_tile_by_work<FEW_T>(p, a.G, a.causal, a.window, un.tile);
     if (at.s < 0) return;
     const int nq = at.q.n * a.G, f0 = at.tile * FEW_T, f1 = min(f0 + FEW_T, nq) - 1;
     const part_at pt = part_of(pg_tiles(at.q, f0, f1, a.G, a.causal, a.window), blockIdx.y, a.chunk, a.parts);
@@ -188,11 +359,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
                     amax = fmaxf(amax, fabsf(e[k]));
                 }
             }
-            // the row is brought to 2^8 .. 2^9 by a power of two, so that the second terms keep their bits
-            amax = quad_max(amax);
-            int ex = 0;
-            if (amax > 0.0f && amax <= 3.402823466e38f) (void)frexpf(amax, &ex);
-            ex = amax > 0.0f && amax <= 3.402823466e38f ? ex - 9 : 0;
+            const int ex = q_exponent(quad_max(amax));
             sc = ldexpf(sc, ex);
 #pragma unroll
             for (int s = 0; s < KS; s++)
@@ -209,35 +376,72 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
         }
     }
 
+    if (threadIdx.x < MAP_BITS / 32) map.w[threadIdx.x] = 0;
+    __syncthreads();
     float m = -INFINITY, l = 0.0f;
     float4v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
 
-    for (int t = pt.t0 + wv; t < pt.t1; t += 4) {
-        const int64_t kb = pg_block(p, at.s, un.kvh, 64 * t + 16 * (i >> 2));
-        const int64_t vb = pg_block(p, at.s, un.kvh, 64 * t + 16 * g);
-        // tokens of the lane's block that exist
-        const int have = vb < 0 ? 0 : pg_clamp(keys - (64 * t + 16 * g), 0, 16);
-        float ks = 1.0f, vs = 1.0f;
-        if constexpr (F8) {
-            if (kb >= 0) ks = p.scale[2 * kb];
-            if (vb >= 0) vs = p.scale[2 * vb + 1];
-        }
-        constexpr int CB = F8 ? 1 : 2;
-        // blocks that do not exist are read at block 0 and not used
-        const uint8_t * kp = (const uint8_t *)p.k + ((kb < 0 ? 0 : kb) * (16 * HD) + (i & 3) * HD + (F8 ? 16 : 8) * g) * CB;
-        const uint8_t * vp = (const uint8_t *)p.v + ((vb < 0 ? 0 : vb) * (16 * HD) + i * 16) * CB;
-        u32x4 kr[4][KW], vr[DT][VW];
+    // Q is waited for here, not inside the loop (where the wait would be for the next tile's loads)
+#pragma unroll
+    for (int c = 0; c < KS; c++) {
+        asm volatile("" : "+v"(qh[c]));
+        if constexpr (F32) asm volatile("" : "+v"(ql[c]));
+    }
+
+    // Keys and values take turns in the same registers: the tile's values are loaded when its scores are
+    // taken, the next tile's keys when the values are added.  That leaves room for four workgroups per CU
+    // (F8), whose waves hide each other's loads; the next tile's pages are looked up a tile earlier.
+    constexpr int CB = F8 ? 1 : 2;
+    const int bs = p.page_shift - 4;                                // log2 of a page's blocks
+    int page_k = -1, page_v = -1, have = 0;
+    float ks = 1.0f, vs = 1.0f;
+    static_assert(4 * KW == DT * VW, "keys and values of a tile");
+    u32x4 cells[4 * KW];
+    auto page_of = [&](int pos) __attribute__((always_inline)) {
+        const int pg = pos < p.cap ? p.pages[(int64_t)at.s * p.ld_pages + (pos >> p.page_shift)] : -1;
+        return pg < p.n_pages ? pg : -1;
+    };
+    // block of the cache; where there is no page, block 0: read and not used
+    auto block_of = [&](int pg, int blk) __attribute__((always_inline)) {
+        return pg < 0 ? (int64_t)0 : (((int64_t)pg * p.Hkv + un.kvh) << bs) + (blk & ((1 << bs) - 1));
+    };
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+        if (t >= pt.t1) return;
+        page_k = page_of(64 * t + 16 * (i >> 2));
+        page_v = page_of(64 * t + 16 * g);
+    };
+    auto load_k = [&](int t) __attribute__((always_inline)) {
+        const int64_t blk = block_of(page_k, 4 * t + (i >> 2));
+        const uint8_t * kp = (const uint8_t *)p.k + (blk * (16 * HD) + (i & 3) * HD + (F8 ? 16 : 8) * g) * CB;
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
-            for (int w = 0; w < KW; w++) kr[u][w] = *(const u32x4 *)(kp + 4 * u * HD * CB + 64 * w);
+            for (int w = 0; w < KW; w++) cells[u * KW + w] = *(const u32x4 *)(kp + 4 * u * HD * CB + 64 * w);
+        if constexpr (F8) ks = p.scale[2 * blk];
+    };
+    auto load_v = [&](int t) __attribute__((always_inline)) {
+        const int64_t blk = block_of(page_v, 4 * t + g);
+        const uint8_t * vp = (const uint8_t *)p.v + (blk * (16 * HD) + i * 16) * CB;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int w = 0; w < VW; w++) vr[d][w] = *(const u32x4 *)(vp + (d * 16 * 16) * CB + 16 * w);
-
+            for (int w = 0; w < VW; w++) cells[d * VW + w] = *(const u32x4 *)(vp + (d * 16 * 16) * CB + 16 * w);
+        have = page_v < 0 ? 0 : pg_clamp(keys - (64 * t + 16 * g), 0, 16);   // tokens of the lane's block that exist
+        if constexpr (F8) {
+            vs = p.scale[2 * blk + 1];
+            if (page_v < 0) vs = 1.0f;
+        }
+    };
+    {
+        const int t = pt.t0 + wv;
+        if (t < pt.t1) {
+            look_up(t);
+            load_k(t);
+        }
+    }
+    for (int t = pt.t0 + wv; t < pt.t1; t += 4) {
         float s[16];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -245,7 +449,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
 #pragma unroll
             for (int w = 0; w < KW; w++) {
                 if constexpr (F8) {
-                    const half8 k0 = f8_half8(kr[u][w].x, kr[u][w].y, ks), k1 = f8_half8(kr[u][w].z, kr[u][w].w, ks);
+                    const half8 k0 = f8_half8(cells[u * KW + w].x, cells[u * KW + w].y, ks), k1 = f8_half8(cells[u * KW + w].z, cells[u * KW + w].w, ks);
                     acc = mfma16(k0, qh[2 * w], acc);
                     acc = mfma16(k1, qh[2 * w + 1], acc);
                     if constexpr (F32) {
@@ -253,7 +457,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
                         acc = mfma16(k1, ql[2 * w + 1], acc);
                     }
                 } else {
-                    const half8 k0 = __builtin_bit_cast(half8, kr[u][w]);
+                    const half8 k0 = __builtin_bit_cast(half8, cells[u * KW + w]);
                     acc = mfma16(k0, qh[w], acc);
                     if constexpr (F32) acc = mfma16(k0, ql[w], acc);
                 }
@@ -261,15 +465,15 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
 #pragma unroll
             for (int r = 0; r < 4; r++) s[4 * u + r] = acc[r] * sc;
         }
+        load_v(t);
+        look_up(t + 4);
         // every key of the tile is there and every query sees it
         const bool full = __all(have == 16) && 64 * t >= all_lo && 64 * t + 63 <= all_hi;
-        uint32_t vis = 0xffffu;                                     // of this lane's 16 tokens
         if (!full) {
             const int k0 = 64 * t + 16 * g;
             const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, have), 0, 16);
-            vis = hi > lo ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
 #pragma unroll
-            for (int k = 0; k < 16; k++) s[k] = (vis >> k) & 1u ? s[k] : -INFINITY;
+            for (int k = 0; k < 16; k++) s[k] = k >= lo && k < hi ? s[k] : -INFINITY;
         }
         float tm = s[0];
 #pragma unroll
@@ -312,11 +516,11 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
                             constexpr int PER = F8 ? 4 : 2;          // tokens per word
                             const int n = have - PER * (4 * w + c);  // of which exist
                             const uint32_t keep = n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
-                            vr[d][w][c] &= keep;
+                            cells[d * VW + w][c] &= keep;
                         }
             }
         }
-        bool special = false;
+        // NaN codes that every query sees are right as they are
         if (!full || !F8) {
             uint32_t sp = 0;
 #pragma unroll
@@ -324,32 +528,26 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
 #pragma unroll
                 for (int w = 0; w < VW; w++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) sp |= special_bits<F8>(vr[d][w][c]);
-            special = __any(sp != 0);
-        }
-        half8 vis_h[2];
-        if (special)
+                    for (int c = 0; c < 4; c++) sp |= special_bits<F8>(cells[d * VW + w][c]);
+            if (__any(sp != 0)) {
+                if (lane == 0) map.note(t - pt.t0);
 #pragma unroll
-            for (int k = 0; k < 16; k++) vis_h[k >> 3][k & 7] = (half_t)(float)((vis >> k) & 1u);
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int w = 0; w < VW; w++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) cells[d * VW + w][c] = without_special<F8>(cells[d * VW + w][c]);
+            }
+        }
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             half8 v0, v1;
             if constexpr (F8) {
-                v0 = f8_half8(vr[d][0].x, vr[d][0].y, vs);
-                v1 = f8_half8(vr[d][0].z, vr[d][0].w, vs);
+                v0 = f8_half8(cells[d * VW].x, cells[d * VW].y, vs);
+                v1 = f8_half8(cells[d * VW].z, cells[d * VW].w, vs);
             } else {
-                v0 = __builtin_bit_cast(half8, vr[d][0]);
-                v1 = __builtin_bit_cast(half8, vr[d][1]);
-            }
-            float4v marks = {0.f, 0.f, 0.f, 0.f};
-            if (special) {
-                half8 m0, m1, n0, n1;
-                split_special(v0, n0, m0);
-                split_special(v1, n1, m1);
-                v0 = n0;
-                v1 = n1;
-                marks = mfma16(m0, vis_h[0], marks);
-                marks = mfma16(m1, vis_h[1], marks);
+                v0 = __builtin_bit_cast(half8, cells[d * VW]);
+                v1 = __builtin_bit_cast(half8, cells[d * VW + VW - 1]);
             }
             o[d] = mfma16(v0, ph[0], o[d]);
             o[d] = mfma16(v1, ph[1], o[d]);
@@ -357,10 +555,8 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
                 o[d] = mfma16(v0, pl[0], o[d]);
                 o[d] = mfma16(v1, pl[1], o[d]);
             }
-            if (special)
-#pragma unroll
-                for (int r = 0; r < 4; r++) o[d][r] += special_of(marks[r]);
         }
+        if (t + 4 < pt.t1) load_k(t + 4);
     }
 
     // ---- the four waves' results
@@ -372,34 +568,618 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
 #pragma unroll
     for (int d = 0; d < DT; d++) *(float4v *)&so[wv][i][16 * d + 4 * g] = o[d];
     __syncthreads();
-    for (int e = threadIdx.x; e < FEW_T * (HD / 4); e += 256) {
-        const int c = e / (HD / 4), d = 4 * (e % (HD / 4)), fc = f0 + c;
-        if (fc > f1) continue;
-        const float mx = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
-        float sum = 0.0f;
-        float4v v = {0.f, 0.f, 0.f, 0.f};
+    join_waves<HD, F8, F32, FEW_T>(p, a, at, pt, un.kvh, f0, f1, &so[0][0][0], &sm[0][0], &sl[0][0], map);
+}
+
+// ---------------------------------------------------------------------------
+// Some rows: 32 queries per workgroup, keys straight from memory
+// ---------------------------------------------------------------------------
+// k_paged_few with the wider product (32 x 32): four waves take the key steps of the workgroup's range
+// in turn and join through LDS.  A step is KT keys, 64 in 8 bits, 32 in f16 (registers).  Lane (i, h) = (lane % 32, lane / 32), rows of the S^T tiles as
+// in k_paged_many: a lane's 16 D values of tile u are the tokens of block 2u + h in order.
+#define MID_T 32
+template <int HD, bool F8, bool F32>
+__global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_mid(paged_t p, attn_t a) {
+    constexpr int U = F8 ? 2 : 1, KT = 32 * U;
+    constexpr int QS = HD / 16, DT = HD / 32;
+    constexpr int KW = F8 ? HD / 32 : HD / 16;  // 16-byte loads of a lane per S tile
+    constexpr int VW = F8 ? 1 : 2;              // 16-byte loads of a lane per O tile and S tile
+    constexpr int CB = F8 ? 1 : 2;
+    constexpr int OS = HD + 4;                  // LDS floats per query
+    extern __shared__ __attribute__((aligned(16))) float so[];              // [4][MID_T][OS]
+    __shared__ float sm[4][MID_T], sl[4][MID_T];
+    __shared__ special_map map;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
+    const unit_at un = unit_of(blockIdx.x, p.Hkv, a.tiles);
+    if (un.kvh >= p.Hkv) return;
+    const tile_at at = wave_tile_by_work<MID_T>(p, a.G, a.causal, a.window, un.tile);
+    if (at.s < 0) return;
+    const int nq = at.q.n * a.G, f0 = at.tile * MID_T, f1 = min(f0 + MID_T, nq) - 1;
+    const part_at pt = part_of(pg_tiles(at.q, f0, f1, a.G, a.causal, a.window), blockIdx.y, a.chunk, a.parts);
+    if ((int)blockIdx.y >= pt.parts) return;
+    const int keys = at.q.keys, p0 = keys - at.q.n;
+    const int all_lo = pg_seen(p0 + f1 / a.G, keys, a.causal, a.window).lo;
+    const int all_hi = pg_seen(p0 + f0 / a.G, keys, a.causal, a.window).hi;
+    const int f = min(f0 + i, f1), row = at.q.r0 + f / a.G, head = un.kvh * a.G + f % a.G;
+    const seen_t me = pg_seen(p0 + f / a.G, keys, a.causal, a.window);
+
+    // ---- Q: step c holds dims in the order in which the lane's key loads bring them
+    half8 qh[QS], ql[F32 ? QS : 1];
+    float sc = LOG2E_F / sqrtf((float)HD);
+    {
+        const int64_t qo = ((int64_t)row * a.H + head) * HD;
+        auto dim = [&](int c) { return F8 ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h; };
+        if constexpr (F32) {
+            float x[QS][8];
+            float amax = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float r = sm[w][c] == -INFINITY ? (sl[w][c] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(sm[w][c] - mx);
-            sum += r * sl[w][c];
-            const float4v x = *(const float4v *)&so[w][c][d];
+            for (int c = 0; c < QS; c++) {
+                const float * src = (const float *)a.q + qo + dim(c);
+                const float4 u = *(const float4 *)src, v = *(const float4 *)(src + 4);
+                const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = fmaf(r, x[k], v[k]);
-        }
-        const int64_t rh = (int64_t)(at.q.r0 + fc / a.G) * a.H + un.kvh * a.G + fc % a.G;
-        if (F32) v *= 1.0f / 16384.0f;
-        if (pt.parts == 1) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            v *= inv;
-            if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + d) = v;
-            else *(half4 *)((half_t *)a.out + rh * HD + d) = half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
-        } else {
-            const int64_t at_part = (int64_t)blockIdx.y * p.n_rows * a.H + rh;
-            *(float4v *)(a.part_o + at_part * HD + d) = v;
-            if (d == 0) {
-                a.part_ml[2 * at_part] = mx;
-                a.part_ml[2 * at_part + 1] = sum;
+                for (int k = 0; k < 8; k++) {
+                    x[c][k] = e[k];
+                    amax = fmaxf(amax, fabsf(e[k]));
+                }
             }
+            const int ex = q_exponent(half_max(amax));
+            sc = ldexpf(sc, ex);
+#pragma unroll
+            for (int c = 0; c < QS; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    half_t hi, lo;
+                    split16(ldexpf(x[c][k], -ex), hi, lo);
+                    qh[c][k] = hi;
+                    ql[c][k] = lo;
+                }
+        } else {
+#pragma unroll
+            for (int c = 0; c < QS; c++) qh[c] = *(const half8 *)((const half_t *)a.q + qo + dim(c));
+        }
+    }
+    if (threadIdx.x < MAP_BITS / 32) map.w[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < QS; c++) {                                  // waited for here, as in k_paged_few
+        asm volatile("" : "+v"(qh[c]));
+        if constexpr (F32) asm volatile("" : "+v"(ql[c]));
+    }
+
+    const int bs = p.page_shift - 4;
+    const int s0 = pt.t0 * (64 / KT), s1 = pt.t1 * (64 / KT);       // key steps
+    int page_k[U], page_v[U], have[U];
+    float ks[U], vs[U];
+    static_assert(KW == DT * VW, "keys and values of a step");
+    u32x4 cells[U][KW];                                             // keys, then values, as in k_paged_few
+    auto page_of = [&](int pos) __attribute__((always_inline)) {
+        const int pg = pos < p.cap ? p.pages[(int64_t)at.s * p.ld_pages + (pos >> p.page_shift)] : -1;
+        return pg < p.n_pages ? pg : -1;
+    };
+    auto block_of = [&](int pg, int blk) __attribute__((always_inline)) {
+        return pg < 0 ? (int64_t)0 : (((int64_t)pg * p.Hkv + un.kvh) << bs) + (blk & ((1 << bs) - 1));
+    };
+    // blocks (counted over the sequence) of the lane's key row and of its values in tile u of step s
+    auto blk_k = [&](int s, int u) { return s * (KT / 16) + 2 * u + ((i >> 2) & 1); };
+    auto blk_v = [&](int s, int u) { return s * (KT / 16) + 2 * u + h; };
+    auto look_up = [&](int s) __attribute__((always_inline)) {
+        if (s >= s1) return;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            page_k[u] = page_of(16 * blk_k(s, u));
+            page_v[u] = page_of(16 * blk_v(s, u));
+        }
+    };
+    auto load_k = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t blk = block_of(page_k[u], blk_k(s, u));
+            const uint8_t * kp = (const uint8_t *)p.k + (blk * 16 + 4 * (i >> 3) + (i & 3)) * (HD * CB) + 16 * h;
+#pragma unroll
+            for (int w = 0; w < KW; w++) cells[u][w] = *(const u32x4 *)(kp + 32 * w);
+            ks[u] = 1.0f;
+            if constexpr (F8) ks[u] = p.scale[2 * blk];
+        }
+    };
+    auto load_v = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t blk = block_of(page_v[u], blk_v(s, u));
+            const uint8_t * vp = (const uint8_t *)p.v + (blk * HD + i) * (16 * CB);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int w = 0; w < VW; w++) cells[u][d * VW + w] = *(const u32x4 *)(vp + 32 * d * 16 * CB + 16 * w);
+            have[u] = page_v[u] < 0 ? 0 : pg_clamp(keys - 16 * blk_v(s, u), 0, 16);
+            vs[u] = 1.0f;
+            if constexpr (F8) {
+                vs[u] = p.scale[2 * blk + 1];
+                if (page_v[u] < 0) vs[u] = 1.0f;
+            }
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    float16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    if (s0 + wv < s1) {
+        look_up(s0 + wv);
+        load_k(s0 + wv);
+    }
+    for (int st = s0 + wv; st < s1; st += 4) {
+        float16v s[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KW; w++) {
+                if constexpr (F8) {
+                    const half8 k0 = f8_half8(cells[u][w].x, cells[u][w].y, ks[u]), k1 = f8_half8(cells[u][w].z, cells[u][w].w, ks[u]);
+                    s[u] = mfma32(k0, qh[2 * w], s[u]);
+                    s[u] = mfma32(k1, qh[2 * w + 1], s[u]);
+                    if constexpr (F32) {
+                        s[u] = mfma32(k0, ql[2 * w], s[u]);
+                        s[u] = mfma32(k1, ql[2 * w + 1], s[u]);
+                    }
+                } else {
+                    const half8 k0 = __builtin_bit_cast(half8, cells[u][w]);
+                    s[u] = mfma32(k0, qh[w], s[u]);
+                    if constexpr (F32) s[u] = mfma32(k0, ql[w], s[u]);
+                }
+            }
+        }
+        load_v(st);
+        look_up(st + 4);
+        bool there = true;
+#pragma unroll
+        for (int u = 0; u < U; u++) there &= have[u] == 16;
+        const bool full = __all(there) && KT * st >= all_lo && KT * st + KT - 1 <= all_hi;
+        if (!full) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k0 = 16 * blk_v(st, u);
+                const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, have[u]), 0, 16);
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[u][r] = r >= lo && r < hi ? s[u][r] : -INFINITY;
+            }
+        }
+        float tm = s[0][0];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) tm = fmaxf(tm, s[u][r]);
+        tm = fmaxf(half_max(tm) * sc, m);
+        if (__any(tm > m)) {
+            const float r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - tm);
+            l *= r;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= r;
+            m = tm;
+        }
+        // 2^14 p goes into the products, as in k_paged_few
+        const float mm = (F32 ? 0.0f : 14.0f) - (m == -INFINITY ? 0.0f : m);
+        half8 ph[2 * U], pl[F32 ? 2 * U : 1];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, mm));
+                l += e;
+                if constexpr (F32) {
+                    half_t hi, lo;
+                    split16(e * 16384.0f, hi, lo);
+                    ph[2 * u + (r >> 3)][r & 7] = hi;
+                    pl[2 * u + (r >> 3)][r & 7] = lo;
+                } else {
+                    ph[2 * u + (r >> 3)][r & 7] = (half_t)e;
+                }
+            }
+        if (!full) {
+            // cells of tokens that do not exist are taken as 0
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int w = 0; w < VW; w++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            constexpr int PER = F8 ? 4 : 2;
+                            const int n = have[u] - PER * (4 * w + c);
+                            cells[u][d * VW + w][c] &= n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
+                        }
+        }
+        if (!full || !F8) {                                         // NaN codes that all see are right as they are
+            uint32_t sp = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int w = 0; w < VW; w++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) sp |= special_bits<F8>(cells[u][d * VW + w][c]);
+            if (__any(sp != 0)) {
+                if (lane == 0) map.note(st / (64 / KT) - pt.t0);
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int w = 0; w < VW; w++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) cells[u][d * VW + w][c] = without_special<F8>(cells[u][d * VW + w][c]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    half8 v;
+                    if constexpr (F8)
+                        v = j ? f8_half8(cells[u][d * VW].z, cells[u][d * VW].w, vs[u]) : f8_half8(cells[u][d * VW].x, cells[u][d * VW].y, vs[u]);
+                    else
+                        v = __builtin_bit_cast(half8, cells[u][d * VW + j]);
+                    o[d] = mfma32(v, ph[2 * u + j], o[d]);
+                    if constexpr (F32) o[d] = mfma32(v, pl[2 * u + j], o[d]);
+                }
+        if (st + 4 < s1) load_k(st + 4);
+    }
+
+    // ---- the four waves' results
+    l = half_sum(l);
+    if (h == 0) {
+        sm[wv][i] = m;
+        sl[wv][i] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+            *(float4v *)&so[(wv * MID_T + i) * OS + 32 * d + 8 * b + 4 * h] =
+                float4v{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+    __syncthreads();
+    join_waves<HD, F8, F32, MID_T>(p, a, at, pt, un.kvh, f0, f1, so, &sm[0][0], &sl[0][0], map);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: 32 queries per wave, keys through LDS
+// ---------------------------------------------------------------------------
+// Bound by the matrix cores and the exponentials.  Four waves share tiles of 64 keys in LDS, in f16 (so an
+// E4M3 cell is converted once for all of them), two buffers: while a tile is multiplied, the next
+// one's cells are on their way to registers; one barrier per tile.  Lane (i, h) = (lane % 32,
+// lane / 32): query column i; S^T tile u (32 of the 64 keys): row 8a + 4b + r is token 4a + r of block
+// 2u + b, so the lane's 16 D values are the 16 tokens of block 2u + h in order.
+// LDS: K by 8-dim chunks, [HD / 8][64 tokens in S^T row order][16 B]; V by halves of blocks,
+// [4 blocks][2][HD][16 B]: every operand read is 64 lanes of consecutive 16 bytes per half wave.
+// The running maximum is let lag (by up to 2^8): sums are rescaled only where it moves further.
+template <int HD> struct many_lds {
+    static constexpr int KS = 64 * 16 + 16;             // bytes per key chunk (the rest of a bank row: writes spread)
+    static constexpr int VS = HD * 16 + 64;             // bytes per half block of values
+    static constexpr int K = (HD / 8) * KS, V = 8 * VS;
+    static constexpr int FLAGS = 2 * 4 * 4 + (int)sizeof(special_map);   // per buffer: 4 counts of tokens
+    static constexpr int BYTES = 2 * (K + V) + FLAGS;
+};
+
+#define MANY_WAVES 4
+#define MANY_T (32 * MANY_WAVES)
+template <int HD, bool F8, bool F32>
+__global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, attn_t a) {
+    constexpr int NT = 64 * MANY_WAVES, T = 32 * MANY_WAVES;
+    constexpr int CB = F8 ? 1 : 2;
+    constexpr int QS = HD / 16;                         // 16-dim steps of S
+    constexpr int DT = HD / 32;                         // 32-dim tiles of O
+    constexpr int UNITS = 64 * HD * CB / 16;            // 16-byte units of a tile of K (as many of V)
+    constexpr int LU = UNITS / NT;                      // of them per thread
+    constexpr int PER_BLOCK = UNITS / 4;
+    using lds_t = many_lds<HD>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    int * flags = (int *)(lds + 2 * (lds_t::K + lds_t::V));      // [2][4]
+    special_map & map = *(special_map *)(flags + 8);
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
+    const unit_at un = unit_of(blockIdx.x, p.Hkv, a.tiles);
+    if (un.kvh >= p.Hkv) return;
+    const tile_at at = wave_tile_by_work<T>(p, a.G, a.causal, a.window, un.tile);
+    if (at.s < 0) return;
+    const int nq = at.q.n * a.G;
+    const int f0 = at.tile * T, f1 = min(f0 + T, nq) - 1;
+    const part_at pt = part_of(pg_tiles(at.q, f0, f1, a.G, a.causal, a.window), blockIdx.y, a.chunk, a.parts);
+    if ((int)blockIdx.y >= pt.parts) return;
+    const int keys = at.q.keys, p0 = keys - at.q.n;
+    // this wave's queries, the keys that all and that any of them see
+    const int w0 = f0 + 32 * wv, w1 = min(w0 + 31, f1);
+    const bool idle = w0 > f1;
+    const seen_t first = pg_seen(p0 + min(w0, f1) / a.G, keys, a.causal, a.window);
+    const seen_t last = pg_seen(p0 + max(w1, 0) / a.G, keys, a.causal, a.window);
+    const int f = min(w0 + i, f1), row = at.q.r0 + f / a.G, head = un.kvh * a.G + f % a.G;
+    const seen_t me = pg_seen(p0 + f / a.G, keys, a.causal, a.window);
+
+    half8 qh[QS], ql[F32 ? QS : 1];
+    float sc = LOG2E_F / sqrtf((float)HD);
+    {
+        const int64_t qo = ((int64_t)row * a.H + head) * HD + 8 * h;
+        if constexpr (F32) {
+            float x[QS][8];
+            float amax = 0.0f;
+#pragma unroll
+            for (int s = 0; s < QS; s++) {
+                const float * src = (const float *)a.q + qo + 16 * s;
+                const float4 u = *(const float4 *)src, v = *(const float4 *)(src + 4);
+                const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    x[s][k] = e[k];
+                    amax = fmaxf(amax, fabsf(e[k]));
+                }
+            }
+            const int ex = q_exponent(half_max(amax));
+            sc = ldexpf(sc, ex);
+#pragma unroll
+            for (int s = 0; s < QS; s++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    half_t hi, lo;
+                    split16(ldexpf(x[s][k], -ex), hi, lo);
+                    qh[s][k] = hi;
+                    ql[s][k] = lo;
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < QS; s++) qh[s] = *(const half8 *)((const half_t *)a.q + qo + 16 * s);
+        }
+    }
+
+    // Q is waited for here, not by the loop's first products (whose wait would be for the loads of the
+    // next tile in every later turn)
+#pragma unroll
+    for (int c = 0; c < QS; c++) {
+        asm volatile("" : "+v"(qh[c]));
+        if constexpr (F32) asm volatile("" : "+v"(ql[c]));
+    }
+
+    // ---- loader: this thread's 16-byte units of a tile; a unit's block is the same for its whole wave.
+    // Pages are looked up a tile ahead: lane 2b + side (mod 8) holds the page of block b and, with the
+    // cells, loads its scale of that side.
+    u32x4 kr[LU], vr[LU];
+    int have[LU], page = -1;
+    float scale = 1.0f;
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+        const int pos = 64 * t + 16 * ((lane >> 1) & 3);
+        page = -1;
+        if (t < pt.t1 && pos < p.cap) page = p.pages[(int64_t)at.s * p.ld_pages + (pos >> p.page_shift)];
+        if (page >= p.n_pages) page = -1;
+    };
+    const int bs = p.page_shift - 4;                    // log2 of a page's blocks
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int w = 0; w < LU; w++) {
+            const int u = tid + NT * w, b = (64 * wv + NT * w) / PER_BLOCK, in = u % PER_BLOCK;
+            const int pg = __builtin_amdgcn_readlane(page, 2 * b);
+            // no page: block 0 of the cache, not used
+            const int64_t blk = pg < 0 ? 0 : (((int64_t)pg * p.Hkv + un.kvh) << bs) + ((4 * t + b) & ((1 << bs) - 1));
+            kr[w] = ((const u32x4 *)p.k)[blk * PER_BLOCK + in];
+            vr[w] = ((const u32x4 *)p.v)[blk * PER_BLOCK + in];
+            have[w] = pg < 0 ? 0 : pg_clamp(keys - 64 * t - 16 * b, 0, 16);
+        }
+        if constexpr (F8) {
+            const int64_t blk = (((int64_t)max(page, 0) * p.Hkv + un.kvh) << bs) + ((4 * t + ((lane >> 1) & 3)) & ((1 << bs) - 1));
+            scale = p.scale[2 * blk + (lane & 1)];
+            scale = page < 0 ? 1.0f : scale;
+        }
+        look_up(t + 1);
+    };
+    auto store = [&](int buf, int t) __attribute__((always_inline)) {
+        uint8_t * kl = lds + buf * (lds_t::K + lds_t::V), * vl = kl + lds_t::K;
+#pragma unroll
+        for (int w = 0; w < LU; w++) {
+            const int u = tid + NT * w, b = (64 * wv + NT * w) / PER_BLOCK, in = u % PER_BLOCK;
+            // keys: token and 16 bytes of its row -> row of S^T tile, chunks
+            constexpr int ROW = HD * CB / 16;                                // units per token
+            const int tok = in / ROW, c = in % ROW;
+            const int slot = 32 * (b >> 1) + 8 * (tok >> 2) + 4 * (b & 1) + (tok & 3);
+            const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 2 * b));
+            const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 2 * b + 1));
+            if constexpr (F8) {
+                *(half8 *)(kl + (2 * c) * lds_t::KS + slot * 16) = f8_half8(kr[w].x, kr[w].y, ks);
+                *(half8 *)(kl + (2 * c + 1) * lds_t::KS + slot * 16) = f8_half8(kr[w].z, kr[w].w, ks);
+            } else {
+                *(u32x4 *)(kl + c * lds_t::KS + slot * 16) = kr[w];
+            }
+            // values: cells of tokens that do not exist are taken as 0
+            if (have[w] < 16) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    constexpr int PER = F8 ? 4 : 2;                          // tokens per word
+                    const int n = have[w] - PER * (4 * (F8 ? 0 : in & 1) + k);
+                    vr[w][k] &= n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
+                }
+            }
+            uint32_t sp = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) sp |= special_bits<F8>(vr[w][k]);
+            if (sp) {
+                map.note(t - pt.t0);
+#pragma unroll
+                for (int k = 0; k < 4; k++) vr[w][k] = without_special<F8>(vr[w][k]);
+            }
+            if constexpr (F8) {
+                *(half8 *)(vl + (2 * b) * lds_t::VS + in * 16) = f8_half8(vr[w].x, vr[w].y, vs);
+                *(half8 *)(vl + (2 * b + 1) * lds_t::VS + in * 16) = f8_half8(vr[w].z, vr[w].w, vs);
+            } else {
+                *(u32x4 *)(vl + (2 * b + (in & 1)) * lds_t::VS + (in >> 1) * 16) = vr[w];
+            }
+            if (in == 0) flags[4 * buf + b] = have[w];
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    float16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+
+    if (tid < MAP_BITS / 32) map.w[tid] = 0;
+    __syncthreads();
+    if (pt.t0 < pt.t1) {
+        look_up(pt.t0);
+        load(pt.t0);
+        store(0, pt.t0);
+    }
+    __syncthreads();
+    for (int t = pt.t0; t < pt.t1; t++) {
+        const int buf = (t - pt.t0) & 1;
+        if (t + 1 < pt.t1) load(t + 1);
+        if (!idle && 64 * t <= last.hi && 64 * t + 63 >= first.lo) {
+            const uint8_t * kl = lds + buf * (lds_t::K + lds_t::V), * vl = kl + lds_t::K;
+            // operands are read ahead of the products that take them, HALF of a side at a time with f32
+            // results (registers)
+            constexpr int KH = QS / 2;
+            float16v s[2];
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
+#pragma unroll
+            for (int c0 = 0; c0 < QS; c0 += KH) {
+                half8 kf[KH][2];
+#pragma unroll
+                for (int c = 0; c < KH; c++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        kf[c][u] = *(const half8 *)(kl + (2 * (c0 + c) + h) * lds_t::KS + (32 * u + i) * 16);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = 0; c < KH; c++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        s[u] = mfma32(kf[c][u], qh[c0 + c], s[u]);
+                        if constexpr (F32) s[u] = mfma32(kf[c][u], ql[c0 + c], s[u]);
+                    }
+            }
+            constexpr int VH = DT / 2;
+            half8 vf[VH][4];
+            auto read_v = [&](int d0) __attribute__((always_inline)) {
+#pragma unroll
+                for (int d = 0; d < VH; d++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++)                              // (u, half) = (g / 2, g % 2)
+                        vf[d][g] = *(const half8 *)(vl + (2 * (2 * (g >> 1) + h) + (g & 1)) * lds_t::VS + (32 * (d0 + d) + i) * 16);
+            };
+            const int4 there = *(const int4 *)(flags + 4 * buf);
+            const bool full = 64 * t >= last.lo && 64 * t + 63 <= first.hi &&
+                              min(min(there.x, there.y), min(there.z, there.w)) == 16;
+            if (!full) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int k0 = 64 * t + 32 * u + 16 * h;
+                    const int n = u == 0 ? (h ? there.y : there.x) : (h ? there.w : there.z);
+                    const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, n), 0, 16);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[u][r] = r >= lo && r < hi ? s[u][r] : -INFINITY;
+                }
+            }
+            // Probabilities against the running maximum as it is; where a lane's sum of them says that one
+            // may leave f16's range, or a query has no maximum yet, the maximum is taken anew and the
+            // sums are brought to it.  2^6 p (f32 results: 2^7 p, applied after the exponential) goes
+            // into the products: small probabilities keep their bits.
+            half8 ph[4], pl[F32 ? 4 : 1];
+            auto weigh = [&]() __attribute__((always_inline)) {
+                const float mm = (F32 ? 0.0f : 6.0f) - (m == -INFINITY ? 0.0f : m);
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, mm));
+                        sum += e;
+                        if constexpr (F32) {
+                            half_t hi, lo;
+                            split16(e * 128.0f, hi, lo);
+                            ph[2 * u + (r >> 3)][r & 7] = hi;
+                            pl[2 * u + (r >> 3)][r & 7] = lo;
+                        } else {
+                            ph[2 * u + (r >> 3)][r & 7] = (half_t)e;
+                        }
+                    }
+                return sum;
+            };
+            float sum = weigh();
+            if (__any(m == -INFINITY || sum > (F32 ? 256.0f : 16384.0f))) {
+                float tm = s[0][0];
+#pragma unroll
+                for (int r = 0; r < 16; r++) tm = fmaxf(tm, fmaxf(s[0][r], s[1][r]));
+                tm = half_max(tm) * sc;
+                const float to = fmaxf(m, tm), r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+                l *= r;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= r;
+                m = to;
+                sum = weigh();
+            }
+            l += sum;
+#pragma unroll
+            for (int d0 = 0; d0 < DT; d0 += VH) {
+                read_v(d0);
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int d = 0; d < VH; d++) {
+                        o[d0 + d] = mfma32(vf[d][g], ph[g], o[d0 + d]);
+                        if constexpr (F32) o[d0 + d] = mfma32(vf[d][g], pl[g], o[d0 + d]);
+                    }
+            }
+        }
+        if (t + 1 < pt.t1) store(buf ^ 1, t + 1);
+        __syncthreads();
+    }
+
+    if (map.any()) {
+        // every wave is past the tiles (the barrier above): their room takes the sums, 32 dims at a time
+        constexpr int OS = 34;
+        static_assert(T * OS * 4 <= 2 * (lds_t::K + lds_t::V), "room for the sums");
+        float * so = (float *)lds + (32 * wv + i) * OS;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) so[8 * (r >> 2) + 4 * h + (r & 3)] = o[d][r];
+#pragma unroll 1
+            for (int e = 0; e < 16; e++) {
+                const int dim = 8 * (e >> 2) + 4 * h + (e & 3);
+                so[dim] += special_sum<HD, F8>(p, map, at.s, un.kvh, 32 * d + dim, pt.t0, pt.t1, me, keys);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = so[8 * (r >> 2) + 4 * h + (r & 3)];
+        }
+    }
+
+    // ---- results: lane's query, dims 32 d + 8 b + 4 h + 0..3 of o[d][4 b ..]
+    if (idle || w0 + i > f1) return;
+    l = half_sum(l);
+    const int64_t rh = (int64_t)row * a.H + head;
+    float mul = F32 ? 1.0f / 128.0f : 1.0f;
+    if (pt.parts == 1) mul = l == 0.0f ? 0.0f : mul / l;
+    const int64_t at_part = (int64_t)blockIdx.y * p.n_rows * a.H + rh;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const int dim = 32 * d + 8 * b + 4 * h;
+            const float4v v = {o[d][4 * b] * mul, o[d][4 * b + 1] * mul, o[d][4 * b + 2] * mul, o[d][4 * b + 3] * mul};
+            if (pt.parts > 1) *(float4v *)(a.part_o + at_part * HD + dim) = v;
+            else if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + dim) = v;
+            else *(half4 *)((half_t *)a.out + rh * HD + dim) = half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+        }
+    if (a.parts > 1 && h == 0) {
+        if (blockIdx.y == 0) a.n_parts[rh] = pt.parts;
+        if (pt.parts > 1) {
+            a.part_ml[2 * at_part] = m;
+            a.part_ml[2 * at_part + 1] = l;
         }
     }
 }
@@ -407,61 +1187,158 @@ __global__ void __launch_bounds__(256, 2) k_paged_few(paged_t p, attn_t a) {
 // ---------------------------------------------------------------------------
 // Joining the parts of a split range
 // ---------------------------------------------------------------------------
-// One workgroup per (row, head): o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i; wave w takes the
-// parts w, w + 4, .. in order, the waves are added in order: the same bits on every run.
-template <int HD, bool F32, int T>
+// o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  W waves per (row, head): half a wave reads a part's
+// sums, HD / 32 dims a lane, so W waves take 2 W parts at a time, all that there may be (ALL of them per
+// half wave) before any is known to be needed: one round of loads.  The sums are added in a fixed
+// order: the same bits on every run.
+template <int HD, bool F32, int W, int ALL>
 __global__ void __launch_bounds__(256) k_paged_join(paged_t p, attn_t a) {
-    constexpr int DL = HD / 64;                 // dims per lane
-    __shared__ float sv[4][HD], ss[4];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int kvh = blockIdx.y, G = a.G;
-    const tile_at at = wave_tile<1>(p, G, blockIdx.x);          // tiles of one query: the flat query itself
-    if (at.s < 0) return;
-    const int nq = at.q.n * G, f0 = at.tile / T * T, f1 = min(f0 + T, nq) - 1;
-    const int parts = part_of(pg_tiles(at.q, f0, f1, G, a.causal, a.window), 0, a.chunk, a.parts).parts;
-    if (parts == 1) return;
-    const int64_t rh = (int64_t)(at.q.r0 + at.tile / G) * a.H + kvh * G + at.tile % G;
-    const int64_t step = (int64_t)p.n_rows * a.H;
-    float mx = -INFINITY;
-    for (int i = lane; i < parts; i += 64) mx = fmaxf(mx, a.part_ml[2 * (i * step + rh)]);
-    mx = wave_max(mx);
-    float sum = 0.0f, v[DL] = {};
-#pragma unroll 4
-    for (int i = wv; i < parts; i += 4) {
-        const float mi = a.part_ml[2 * (i * step + rh)], li = a.part_ml[2 * (i * step + rh) + 1];
-        const float r = mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(mi - mx);
-        sum += r * li;
+    constexpr int DL = HD / 32;                                 // dims per lane
+    __shared__ float sv[4][HD];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5, w = wv % W;
+    const int64_t rows = (int64_t)p.n_rows * a.H, rh = (int64_t)blockIdx.x * (4 / W) + wv / W;
+    if (W < 4 && rh >= rows) return;                            // W = 4: the grid is the rows
+    // rows of no sequence have no parts; the others' number was written with their first part
+    const int row = (int)(rh / a.H);
+    const bool in = row >= p.rows[0] && row < p.rows[p.n_seqs];
+    const int n = a.n_parts[rh];
+    float mi[ALL], v[ALL][DL];
+    const float * src = a.part_o + rh * HD + DL * (lane & 31);
 #pragma unroll
-        for (int k = 0; k < DL; k++) v[k] = fmaf(r, a.part_o[(i * step + rh) * HD + DL * lane + k], v[k]);
+    for (int i = 0; i < ALL; i++) {
+        const int64_t at = (int64_t)min(2 * (w + W * i) + half, a.parts - 1) * rows;
+        mi[i] = a.part_ml[2 * (at + rh)];
+#pragma unroll
+        for (int k = 0; k < DL; k++) v[i][k] = src[at * HD + k];
+    }
+    float m_l = -INFINITY, l_l = 0.0f;                          // lane's part of the row's maximum and sum
+    if (lane < a.parts) {
+        m_l = a.part_ml[2 * (lane * rows + rh)];
+        l_l = a.part_ml[2 * (lane * rows + rh) + 1];
+    }
+    const int parts = in ? min(n, a.parts) : 1;
+    if (parts <= 1) return;                                     // the same for the output's W waves
+    const float mx = wave_max(lane < parts ? m_l : -INFINITY);
+    float sum = lane < parts ? (m_l == -INFINITY ? l_l : __builtin_amdgcn_exp2f(m_l - mx) * l_l) : 0.0f;
+    sum = wave_sum(sum);
+    float t[DL] = {};
+#pragma unroll
+    for (int i = 0; i < ALL; i++) {
+        // held above 0: an infinite sum stays one; a part that saw nothing has zeros, or NaN
+        const float r = mi[i] == -INFINITY ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(mi[i] - mx), 0x1p-126f);
+        const bool is = 2 * (w + W * i) + half < parts;
+#pragma unroll
+        for (int k = 0; k < DL; k++) t[k] = is ? fmaf(r, v[i][k], t[k]) : t[k];
     }
 #pragma unroll
-    for (int k = 0; k < DL; k++) sv[wv][DL * lane + k] = v[k];
-    if (lane == 0) ss[wv] = sum;
-    __syncthreads();
-    if (threadIdx.x < HD) {
-        const int d = threadIdx.x;
-        const float l = (ss[0] + ss[1]) + (ss[2] + ss[3]), x = (sv[0][d] + sv[1][d]) + (sv[2][d] + sv[3][d]);
-        const float y = l == 0.0f ? 0.0f : x * (1.0f / l);
-        if constexpr (F32) ((float *)a.out)[rh * HD + d] = y;
-        else ((half_t *)a.out)[rh * HD + d] = (half_t)y;
+    for (int k = 0; k < DL; k++) t[k] += __shfl_xor(t[k], 32, WAVE);
+    if constexpr (W > 1) {
+        if (half == 0)
+#pragma unroll
+            for (int k = 0; k < DL; k++) sv[wv][DL * lane + k] = t[k];
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int k = 0; k < DL; k++) {
+            t[k] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; j++) t[k] += sv[wv + j][DL * (lane & 31) + k];
+        }
+    }
+    if (half) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int k = 0; k < DL; k++) {
+        const int64_t o = rh * HD + DL * lane + k;
+        if constexpr (F32) ((float *)a.out)[o] = t[k] * inv;
+        else ((half_t *)a.out)[o] = (half_t)(t[k] * inv);
     }
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-struct attn_plan { int tiles, chunk, parts; };
-static attn_plan plan_of(const paged_t & p, int H, int64_t max_keys, bool split) {
+// T: queries per workgroup; 16 is k_paged_few, 32 k_paged_mid, 128 k_paged_many.
+// most: parts that the workspace has room for, whatever the window (fewer key tiles, no more parts).
+struct attn_plan { int T, tiles, chunk, parts, most; };
+// A range is split where a query tile has more than WHOLE key tiles and the workgroups are few: the join
+// costs a launch (12 tiles, 32 heads: 1 row in 8 sequences 16.1 us whole, 18.2 in two parts, 128 rows 15.1 /
+// 19.7; 55 tiles, 4 KV heads, 2 rows: 14.9 in 4 parts, 10.0 in 14).
+#define WHOLE 16
+#define MIN_CHUNK 4    // key tiles of a part: one per wave
+#define MAX_PARTS 64   // a lane each in the join
+static attn_plan plan_of(const paged_t & p, int H, int64_t max_keys, int window, bool split) {
     const int G = H / p.Hkv;
-    const int64_t queries = (int64_t)p.n_rows * G;
+    const int64_t queries = (int64_t)p.n_rows * G, seqs = std::min<int64_t>(p.n_seqs, p.n_rows), all = queries * p.Hkv;
     attn_plan r;
-    r.tiles = (int)(queries / FEW_T + std::min<int64_t>(p.n_seqs, p.n_rows));
-    const int64_t kt = (std::min<int64_t>(std::max<int64_t>(max_keys, 1), p.cap) + 63) / 64;
-    const int64_t units = (int64_t)p.Hkv * std::max<int64_t>(std::min<int64_t>(p.n_seqs, p.n_rows), queries / FEW_T);
-    const int64_t want = std::max<int64_t>(1, 512 / units);
-    r.chunk = (int)std::max<int64_t>(8, (kt + want - 1) / want);
-    r.parts = split ? (int)((kt + r.chunk - 1) / r.chunk) : 1;
+    // The narrow tiles read the keys more often but come in more workgroups, four waves to a range of keys:
+    // they are taken up to two (16 queries) and four (32) workgroups per CU, or where no sequence fills more.
+    // 16 / 32 / 128 queries, us: 4 x 64 rows of 32 heads over 764 f16 keys 26 / 31 / 41, 4 x 128 rows 52 / 35 /
+    // 52, 4 x 512 rows 236 / 160 / 115; 32 rows of 28 heads over 3532 keys 16.3 / 15.6 / 26, 512 rows 85 / 57 / 58,
+    // 1024 rows 144 / 109 / 100; 8 x 32 rows of 32 heads over 732 keys 17 / 27 / 31, 8 x 256 101 / 85 / 57.
+    r.T = queries <= 16 * seqs || all <= 512 * 16 ? FEW_T : queries <= 32 * seqs || all <= 1024 * 32 ? MID_T : MANY_T;
+    r.tiles = (int)(queries / r.T + seqs);
+    const int64_t units = (int64_t)p.Hkv * std::max<int64_t>(seqs, queries / r.T);
+    const int64_t want = std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, 512 / units));
+    // key tiles that a query tile can see
+    int64_t kt = (std::min<int64_t>(std::max<int64_t>(max_keys, 1), p.cap) + 63) / 64;
+    r.most = kt <= WHOLE ? 1 : (int)std::min<int64_t>(want, (kt + MIN_CHUNK - 1) / MIN_CHUNK);
+    if (window > 0) kt = std::min<int64_t>(kt, ((int64_t)window + r.T / G + 63) / 64 + 1);
+    r.chunk = (int)std::max<int64_t>(MIN_CHUNK, (kt + want - 1) / want);
+    r.parts = split && kt > WHOLE ? (int)((kt + r.chunk - 1) / r.chunk) : 1;
     return r;
+}
+
+// More than 64 KB of LDS needs the kernel's limit raised, once per device (`set`: a bit per device).
+static int many_lds_limit(const void * kernel, int bytes, std::atomic<uint64_t> & set) {
+    if (bytes <= 64 * 1024) return DFX_OK;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (set.load(std::memory_order_acquire) >> dev & 1) return DFX_OK;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) {
+        dfx_set_error("dfx_paged_attention: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+        return DFX_ERR_HIP;
+    }
+    set.fetch_or(1ull << dev, std::memory_order_release);
+    return DFX_OK;
+}
+
+template <int HD, bool F8, bool F32>
+static int many_launch(const paged_t & p, const attn_t & a, dim3 grid, hipStream_t st) {
+    static std::atomic<uint64_t> set;
+    constexpr int bytes = many_lds<HD>::BYTES;
+    const int rc = many_lds_limit((const void *)k_paged_many<HD, F8, F32>, bytes, set);
+    if (rc != DFX_OK) return rc;
+    hipLaunchKernelGGL((k_paged_many<HD, F8, F32>), grid, dim3(64 * MANY_WAVES), bytes, st, p, a);
+    return DFX_OK;
+}
+
+template <int HD, bool F8, bool F32>
+static int attn_launch(const paged_t & p, const attn_t & a, const attn_plan & pl, hipStream_t st) {
+    const dim3 grid(unit_grid(p.Hkv, pl.tiles), (unsigned)pl.parts);
+    int rc = DFX_OK;
+    if (pl.T == FEW_T) hipLaunchKernelGGL((k_paged_few<HD, F8, F32>), grid, dim3(256), 0, st, p, a);
+    else if (pl.T == MID_T) {
+        static std::atomic<uint64_t> set;
+        constexpr int bytes = 4 * MID_T * (HD + 4) * (int)sizeof(float);
+        rc = many_lds_limit((const void *)k_paged_mid<HD, F8, F32>, bytes, set);
+        if (rc == DFX_OK) hipLaunchKernelGGL((k_paged_mid<HD, F8, F32>), grid, dim3(256), bytes, st, p, a);
+    }
+    else rc = many_launch<HD, F8, F32>(p, a, grid, st);
+    if (rc != DFX_OK) return rc;
+    DFX_CHECK_LAUNCH("dfx_paged_attention");
+    if (pl.parts > 1) {
+        const int64_t rows = (int64_t)p.n_rows * a.H;
+        if (pl.parts <= 8)
+            hipLaunchKernelGGL((k_paged_join<HD, F32, 1, 4>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, a);
+        else if (pl.parts <= 32)
+            hipLaunchKernelGGL((k_paged_join<HD, F32, 4, 4>), dim3((unsigned)rows), dim3(256), 0, st, p, a);
+        else
+            hipLaunchKernelGGL((k_paged_join<HD, F32, 4, MAX_PARTS / 8>), dim3((unsigned)rows), dim3(256), 0, st, p, a);
+        DFX_CHECK_LAUNCH("dfx_paged_attention (join)");
+    }
+    return DFX_OK;
 }
 
 extern "C" size_t dfx_paged_attention_ws_bytes(const dfx_paged_cache * cache, const dfx_paged_batch * batch, int n_head,
@@ -470,8 +1347,8 @@ extern "C" size_t dfx_paged_attention_ws_bytes(const dfx_paged_cache * cache, co
     (void)type;
     if (paged_of("dfx_paged_attention_ws_bytes", cache, batch, n_head, &p) != DFX_OK) return 0;
     if (p.n_rows == 0 || p.n_seqs == 0) return 0;
-    const attn_plan pl = plan_of(p, n_head, batch->max_keys, true);
-    return pl.parts <= 1 ? 0 : (size_t)pl.parts * p.n_rows * n_head * (cache->head_dim + 2) * sizeof(float);
+    const attn_plan pl = plan_of(p, n_head, batch->max_keys, 0, true);
+    return pl.most <= 1 ? 0 : ((size_t)pl.most * (cache->head_dim + 2) + 1) * p.n_rows * n_head * sizeof(float);
 }
 
 extern "C" int dfx_paged_attention(const dfx_paged_cache * cache, const dfx_paged_batch * batch, const void * q, int type,
@@ -494,36 +1371,15 @@ extern "C" int dfx_paged_attention(const dfx_paged_cache * cache, const dfx_page
         return DFX_ERR_ARG;
     }
     const int hd = cache->head_dim;
-    const attn_plan pl = plan_of(p, n_head, batch->max_keys, ws != nullptr);
-    attn_t a = {q, out, (float *)ws, nullptr, n_head, n_head / p.Hkv, causal ? 1 : 0, window, pl.chunk, pl.parts, pl.tiles};
+    const attn_plan pl = plan_of(p, n_head, batch->max_keys, window, ws != nullptr);
+    attn_t a = {q, out, (float *)ws, nullptr, nullptr, n_head, n_head / p.Hkv, causal ? 1 : 0, window, pl.chunk, pl.parts, pl.tiles};
     a.part_ml = a.part_o + (size_t)pl.parts * p.n_rows * n_head * hd;
+    a.n_parts = (int32_t *)(a.part_ml + (size_t)pl.parts * p.n_rows * n_head * 2);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid(unit_grid(p.Hkv, pl.tiles), (unsigned)pl.parts);
-#define FEW(HD, F8, F32) hipLaunchKernelGGL((k_paged_few<HD, F8, F32>), grid, dim3(256), 0, st, p, a)
-#define FEW_TYPES(HD)                                                                                                 \
-    do {                                                                                                              \
-        if (cache->type == DFX_TYPE_F8) {                                                                             \
-            if (type == DFX_TYPE_F32) FEW(HD, true, true);                                                            \
-            else FEW(HD, true, false);                                                                                \
-        } else {                                                                                                      \
-            if (type == DFX_TYPE_F32) FEW(HD, false, true);                                                           \
-            else FEW(HD, false, false);                                                                               \
-        }                                                                                                             \
-    } while (0)
-    if (hd == 128) FEW_TYPES(128);
-    else FEW_TYPES(64);
-    DFX_CHECK_LAUNCH("dfx_paged_attention");
-    if (pl.parts > 1) {
-        const dim3 jg((unsigned)((int64_t)p.n_rows * a.G), (unsigned)p.Hkv);
-#define JOIN(HD, F32) hipLaunchKernelGGL((k_paged_join<HD, F32, FEW_T>), jg, dim3(256), 0, st, p, a)
-        if (hd == 128) {
-            if (type == DFX_TYPE_F32) JOIN(128, true);
-            else JOIN(128, false);
-        } else {
-            if (type == DFX_TYPE_F32) JOIN(64, true);
-            else JOIN(64, false);
-        }
-        DFX_CHECK_LAUNCH("dfx_paged_attention (join)");
-    }
-    return DFX_OK;
+    const bool f8 = cache->type == DFX_TYPE_F8, f32 = type == DFX_TYPE_F32;
+    const auto launch = hd == 128 ? (f8 ? (f32 ? attn_launch<128, true, true> : attn_launch<128, true, false>)
+                                        : (f32 ? attn_launch<128, false, true> : attn_launch<128, false, false>))
+                                  : (f8 ? (f32 ? attn_launch<64, true, true> : attn_launch<64, true, false>)
+                                        : (f32 ? attn_launch<64, false, true> : attn_launch<64, false, false>));
+    return launch(p, a, pl, st);
 }

@@ -263,6 +263,9 @@ ATTENDS = [
     ([0, 130, 0], [0, 150, 7], 64, 2, 2, 64),
     ([3], [700], 256, 1, 7, 128),
     ([160], [200], 16, 1, 1, 128),
+    ([300], [340], 64, 1, 4, 128),
+    ([40, 3, 0, 21], [90, 70, 64, 21], 16, 3, 2, 64),
+    ([35, 90], [35, 260], 32, 5, 1, 128),
 ]
 
 
@@ -307,8 +310,26 @@ def test_attention_of_long_caches_is_split(gpu, n, keys, f32):
     check_attention(run_attention(c, b, q, H, True, 0), c, b, q, True, 0, f32)
 
 
+@pytest.mark.parametrize("causal,window", [(False, 0), (True, 0), (True, 20)])
+@pytest.mark.parametrize("S,most", [(63, 2), (64, 30), (65, 3), (150, 40), (70, 150)])
+def test_attention_of_many_sequences(gpu, S, most, causal, window):
+    """Ragged batches of up to and beyond 64 sequences, empty ones among them, at rows that take each kernel:
+    every tile of every sequence is computed once."""
+    rng = np.random.default_rng(S + most)
+    Hkv, G, hd, page = 1, 1, 64, 16
+    n = [0 if rng.random() < 0.1 else int(rng.integers(most // 2 + 1, most + 1)) for _ in range(S)]
+    keys = [m + int(rng.integers(0, 80)) for m in n]
+    c = Cache(F8, page, Hkv, hd, sum(-(-k // page) for k in keys))
+    b = Batch(n, keys, page, c.n_pages, pad_rows=3)
+    fill_keys(c, b, rng)
+    q = (rng.standard_normal((b.M, G, hd)) * 1.5).astype(np.float16)
+    got = run_attention(c, b, q, G, causal, window)
+    check_attention(got, c, b, q, causal, window, False)
+    assert (got[int(b.rows[-1]):] == 7.0).all()
+
+
 @pytest.mark.parametrize("typ", [F8, F16])
-@pytest.mark.parametrize("rows", [1, 30, 200])
+@pytest.mark.parametrize("rows", [1, 30, 100, 200])
 def test_attention_never_sees_hidden_keys(gpu, typ, rows):
     """NaN and infinities in keys and values that some rows see and others do not (later positions, left of
     the window), in the same tile: they reach exactly the rows that see them."""
@@ -353,6 +374,18 @@ def test_attention_without_keys_pages_or_rows(gpu, f32):
     b.set(keys=[-5, 1 << 30, 20, -(1 << 31), 4])          # counts out of range are held in it
     for causal in (False, True):
         check_attention(run_attention(c, b, q, H, causal, 0), c, b, q, causal, 0, f32)
+
+
+@pytest.mark.parametrize("rows,keys", [(40, 3), (300, 100), (300, 0), (700, 30)])
+def test_attention_of_more_rows_than_keys(gpu, rows, keys):
+    """Rows before the first position see nothing under the causal mask: zeros, however many."""
+    rng = np.random.default_rng(rows)
+    c = Cache(F8, 16, 1, 64, 12)
+    b = Batch([rows, 5], [keys, 70], 16, 12)
+    fill_keys(c, b, rng)
+    q = rng.standard_normal((b.M, 2, 64)).astype(np.float16)
+    for causal in (True, False):
+        check_attention(run_attention(c, b, q, 2, causal, 0), c, b, q, causal, 0, False)
 
 
 def test_attention_of_extreme_queries(gpu):
