@@ -19,7 +19,7 @@
 #include <atomic>
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 #define LOG2E_F 1.44269504088896341f
 
@@ -378,10 +378,8 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 
     if (threadIdx.x < MAP_BITS / 32) map.w[threadIdx.x] = 0;
     __syncthreads();
-    float m = -INFINITY, l = 0.0f;
+    float m, l;
     float4v o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
 
     // Q is waited for here, not inside the loop (where the wait would be for the next tile's loads)
 #pragma unroll
@@ -434,129 +432,136 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
             if (page_v < 0) vs = 1.0f;
         }
     };
-    {
-        const int t = pt.t0 + wv;
-        if (t < pt.t1) {
-            look_up(t);
-            load_k(t);
+    bool careful = false;                                           // this wave alone: nothing is shared here
+    while (true) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
+        {
+            const int t = pt.t0 + wv;
+            if (t < pt.t1) {
+                look_up(t);
+                load_k(t);
+            }
         }
-    }
-    for (int t = pt.t0 + wv; t < pt.t1; t += 4) {
-        float s[16];
+        for (int t = pt.t0 + wv; t < pt.t1; t += 4) {
+            float s[16];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            float4v acc = {0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < 4; u++) {
+                float4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < KW; w++) {
-                if constexpr (F8) {
-                    const half8 k0 = f8_half8(cells[u * KW + w].x, cells[u * KW + w].y, ks), k1 = f8_half8(cells[u * KW + w].z, cells[u * KW + w].w, ks);
-                    acc = mfma16(k0, qh[2 * w], acc);
-                    acc = mfma16(k1, qh[2 * w + 1], acc);
-                    if constexpr (F32) {
-                        acc = mfma16(k0, ql[2 * w], acc);
-                        acc = mfma16(k1, ql[2 * w + 1], acc);
+                for (int w = 0; w < KW; w++) {
+                    if constexpr (F8) {
+                        const half8 k0 = f8_half8(cells[u * KW + w].x, cells[u * KW + w].y, ks), k1 = f8_half8(cells[u * KW + w].z, cells[u * KW + w].w, ks);
+                        acc = mfma16(k0, qh[2 * w], acc);
+                        acc = mfma16(k1, qh[2 * w + 1], acc);
+                        if constexpr (F32) {
+                            acc = mfma16(k0, ql[2 * w], acc);
+                            acc = mfma16(k1, ql[2 * w + 1], acc);
+                        }
+                    } else {
+                        const half8 k0 = __builtin_bit_cast(half8, cells[u * KW + w]);
+                        acc = mfma16(k0, qh[w], acc);
+                        if constexpr (F32) acc = mfma16(k0, ql[w], acc);
                     }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[4 * u + r] = acc[r] * sc;
+            }
+            load_v(t);
+            look_up(t + 4);
+            // every key of the tile is there and every query sees it
+            const bool full = __all(have == 16) && 64 * t >= all_lo && 64 * t + 63 <= all_hi;
+            if (!full) {
+                const int k0 = 64 * t + 16 * g;
+                const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, have), 0, 16);
+#pragma unroll
+                for (int k = 0; k < 16; k++) s[k] = k >= lo && k < hi ? s[k] : -INFINITY;
+            }
+            float tm = s[0];
+#pragma unroll
+            for (int k = 1; k < 16; k++) tm = fmaxf(tm, s[k]);
+            tm = fmaxf(quad_max(tm), m);
+            if (__any(tm > m)) {
+                const float r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - tm);
+                l *= r;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= r;
+                m = tm;
+            }
+            // 2^14 p goes into the products, in f16: small probabilities keep their bits.  With f16 results
+            // the exponent carries the factor (l has it too); for f32 results it is applied after, as the
+            // exponent's rounding would show.  Nothing seen yet: every p is 0.
+            const float mm = (m == -INFINITY ? 0.0f : m) - (F32 ? 0.0f : 14.0f);
+            half8 ph[2], pl[2];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const float e = __builtin_amdgcn_exp2f(s[k] - mm);
+                l += e;
+                if constexpr (F32) {
+                    half_t hi, lo;
+                    split16(e * 16384.0f, hi, lo);
+                    ph[k >> 3][k & 7] = hi;
+                    pl[k >> 3][k & 7] = lo;
                 } else {
-                    const half8 k0 = __builtin_bit_cast(half8, cells[u * KW + w]);
-                    acc = mfma16(k0, qh[w], acc);
-                    if constexpr (F32) acc = mfma16(k0, ql[w], acc);
+                    ph[k >> 3][k & 7] = (half_t)e;
                 }
             }
+            if (!full) {
+                // cells of tokens that do not exist are taken as 0
+                if (__any(have < 16)) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[4 * u + r] = acc[r] * sc;
-        }
-        load_v(t);
-        look_up(t + 4);
-        // every key of the tile is there and every query sees it
-        const bool full = __all(have == 16) && 64 * t >= all_lo && 64 * t + 63 <= all_hi;
-        if (!full) {
-            const int k0 = 64 * t + 16 * g;
-            const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, have), 0, 16);
+                    for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int k = 0; k < 16; k++) s[k] = k >= lo && k < hi ? s[k] : -INFINITY;
-        }
-        float tm = s[0];
+                        for (int w = 0; w < VW; w++)
 #pragma unroll
-        for (int k = 1; k < 16; k++) tm = fmaxf(tm, s[k]);
-        tm = fmaxf(quad_max(tm), m);
-        if (__any(tm > m)) {
-            const float r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - tm);
-            l *= r;
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[d] *= r;
-            m = tm;
-        }
-        // 2^14 p goes into the products, in f16: small probabilities keep their bits.  With f16 results
-        // the exponent carries the factor (l has it too); for f32 results it is applied after, as the
-        // exponent's rounding would show.  Nothing seen yet: every p is 0.
-        const float mm = (m == -INFINITY ? 0.0f : m) - (F32 ? 0.0f : 14.0f);
-        half8 ph[2], pl[2];
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-            const float e = __builtin_amdgcn_exp2f(s[k] - mm);
-            l += e;
-            if constexpr (F32) {
-                half_t hi, lo;
-                split16(e * 16384.0f, hi, lo);
-                ph[k >> 3][k & 7] = hi;
-                pl[k >> 3][k & 7] = lo;
-            } else {
-                ph[k >> 3][k & 7] = (half_t)e;
+                            for (int c = 0; c < 4; c++) {
+                                constexpr int PER = F8 ? 4 : 2;          // tokens per word
+                                const int n = have - PER * (4 * w + c);  // of which exist
+                                const uint32_t keep = n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
+                                cells[d * VW + w][c] &= keep;
+                            }
+                }
             }
-        }
-        if (!full) {
-            // cells of tokens that do not exist are taken as 0
-            if (__any(have < 16)) {
+            if (careful) {
+                uint32_t sp = 0;
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                for (int c = 0; c < DT * VW; c++)
 #pragma unroll
-                    for (int w = 0; w < VW; w++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            constexpr int PER = F8 ? 4 : 2;          // tokens per word
-                            const int n = have - PER * (4 * w + c);  // of which exist
-                            const uint32_t keep = n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
-                            cells[d * VW + w][c] &= keep;
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        sp |= special_bits<F8>(cells[c][e]);
+                        cells[c][e] = without_special<F8>(cells[c][e]);
+                    }
+                if (sp) map.note(t - pt.t0);
             }
-        }
-        // NaN codes that every query sees are right as they are
-        if (!full || !F8) {
-            uint32_t sp = 0;
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int w = 0; w < VW; w++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) sp |= special_bits<F8>(cells[d * VW + w][c]);
-            if (__any(sp != 0)) {
-                if (lane == 0) map.note(t - pt.t0);
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int w = 0; w < VW; w++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) cells[d * VW + w][c] = without_special<F8>(cells[d * VW + w][c]);
+            for (int d = 0; d < DT; d++) {
+                half8 v0, v1;
+                if constexpr (F8) {
+                    v0 = f8_half8(cells[d * VW].x, cells[d * VW].y, vs);
+                    v1 = f8_half8(cells[d * VW].z, cells[d * VW].w, vs);
+                } else {
+                    v0 = __builtin_bit_cast(half8, cells[d * VW]);
+                    v1 = __builtin_bit_cast(half8, cells[d * VW + VW - 1]);
+                }
+                o[d] = mfma16(v0, ph[0], o[d]);
+                o[d] = mfma16(v1, ph[1], o[d]);
+                if constexpr (F32) {
+                    o[d] = mfma16(v0, pl[0], o[d]);
+                    o[d] = mfma16(v1, pl[1], o[d]);
+                }
             }
+            if (t + 4 < pt.t1) load_k(t + 4);
         }
+        if (careful) break;
+        bool odd = false;
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            half8 v0, v1;
-            if constexpr (F8) {
-                v0 = f8_half8(cells[d * VW].x, cells[d * VW].y, vs);
-                v1 = f8_half8(cells[d * VW].z, cells[d * VW].w, vs);
-            } else {
-                v0 = __builtin_bit_cast(half8, cells[d * VW]);
-                v1 = __builtin_bit_cast(half8, cells[d * VW + VW - 1]);
-            }
-            o[d] = mfma16(v0, ph[0], o[d]);
-            o[d] = mfma16(v1, ph[1], o[d]);
-            if constexpr (F32) {
-                o[d] = mfma16(v0, pl[0], o[d]);
-                o[d] = mfma16(v1, pl[1], o[d]);
-            }
-        }
-        if (t + 4 < pt.t1) load_k(t + 4);
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) odd |= !(fabsf(o[d][r]) <= 3.402823466e38f);
+        if (!__any(odd)) break;
+        careful = true;
     }
 
     // ---- the four waves' results
@@ -700,112 +705,91 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
         }
     };
 
-    float m = -INFINITY, l = 0.0f;
+    float m, l;
     float16v o[DT];
+    bool careful = false;                                           // this wave alone: nothing is shared here
+    while (true) {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    if (s0 + wv < s1) {
-        look_up(s0 + wv);
-        load_k(s0 + wv);
-    }
-    for (int st = s0 + wv; st < s1; st += 4) {
-        float16v s[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < KW; w++) {
-                if constexpr (F8) {
-                    const half8 k0 = f8_half8(cells[u][w].x, cells[u][w].y, ks[u]), k1 = f8_half8(cells[u][w].z, cells[u][w].w, ks[u]);
-                    s[u] = mfma32(k0, qh[2 * w], s[u]);
-                    s[u] = mfma32(k1, qh[2 * w + 1], s[u]);
-                    if constexpr (F32) {
-                        s[u] = mfma32(k0, ql[2 * w], s[u]);
-                        s[u] = mfma32(k1, ql[2 * w + 1], s[u]);
-                    }
-                } else {
-                    const half8 k0 = __builtin_bit_cast(half8, cells[u][w]);
-                    s[u] = mfma32(k0, qh[w], s[u]);
-                    if constexpr (F32) s[u] = mfma32(k0, ql[w], s[u]);
-                }
-            }
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+        if (s0 + wv < s1) {
+            look_up(s0 + wv);
+            load_k(s0 + wv);
         }
-        load_v(st);
-        look_up(st + 4);
-        bool there = true;
-#pragma unroll
-        for (int u = 0; u < U; u++) there &= have[u] == 16;
-        const bool full = __all(there) && KT * st >= all_lo && KT * st + KT - 1 <= all_hi;
-        if (!full) {
+        for (int st = s0 + wv; st < s1; st += 4) {
+            float16v s[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int k0 = 16 * blk_v(st, u);
-                const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, have[u]), 0, 16);
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[u][r] = r >= lo && r < hi ? s[u][r] : -INFINITY;
-            }
-        }
-        float tm = s[0][0];
+                for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) tm = fmaxf(tm, s[u][r]);
-        tm = fmaxf(half_max(tm) * sc, m);
-        if (__any(tm > m)) {
-            const float r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - tm);
-            l *= r;
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[d] *= r;
-            m = tm;
-        }
-        // 2^14 p goes into the products, as in k_paged_few
-        const float mm = (F32 ? 0.0f : 14.0f) - (m == -INFINITY ? 0.0f : m);
-        half8 ph[2 * U], pl[F32 ? 2 * U : 1];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, mm));
-                l += e;
-                if constexpr (F32) {
-                    half_t hi, lo;
-                    split16(e * 16384.0f, hi, lo);
-                    ph[2 * u + (r >> 3)][r & 7] = hi;
-                    pl[2 * u + (r >> 3)][r & 7] = lo;
-                } else {
-                    ph[2 * u + (r >> 3)][r & 7] = (half_t)e;
+                for (int w = 0; w < KW; w++) {
+                    if constexpr (F8) {
+                        const half8 k0 = f8_half8(cells[u][w].x, cells[u][w].y, ks[u]), k1 = f8_half8(cells[u][w].z, cells[u][w].w, ks[u]);
+                        s[u] = mfma32(k0, qh[2 * w], s[u]);
+                        s[u] = mfma32(k1, qh[2 * w + 1], s[u]);
+                        if constexpr (F32) {
+                            s[u] = mfma32(k0, ql[2 * w], s[u]);
+                            s[u] = mfma32(k1, ql[2 * w + 1], s[u]);
+                        }
+                    } else {
+                        const half8 k0 = __builtin_bit_cast(half8, cells[u][w]);
+                        s[u] = mfma32(k0, qh[w], s[u]);
+                        if constexpr (F32) s[u] = mfma32(k0, ql[w], s[u]);
+                    }
                 }
             }
-        if (!full) {
-            // cells of tokens that do not exist are taken as 0
+            load_v(st);
+            look_up(st + 4);
+            bool there = true;
+#pragma unroll
+            for (int u = 0; u < U; u++) there &= have[u] == 16;
+            const bool full = __all(there) && KT * st >= all_lo && KT * st + KT - 1 <= all_hi;
+            if (!full) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int k0 = 16 * blk_v(st, u);
+                    const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, have[u]), 0, 16);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[u][r] = r >= lo && r < hi ? s[u][r] : -INFINITY;
+                }
+            }
+            float tm = s[0][0];
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                for (int r = 0; r < 16; r++) tm = fmaxf(tm, s[u][r]);
+            tm = fmaxf(half_max(tm) * sc, m);
+            if (__any(tm > m)) {
+                const float r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - tm);
+                l *= r;
 #pragma unroll
-                    for (int w = 0; w < VW; w++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            constexpr int PER = F8 ? 4 : 2;
-                            const int n = have[u] - PER * (4 * w + c);
-                            cells[u][d * VW + w][c] &= n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
-                        }
-        }
-        if (!full || !F8) {                                         // NaN codes that all see are right as they are
-            uint32_t sp = 0;
+                for (int d = 0; d < DT; d++) o[d] *= r;
+                m = tm;
+            }
+            // 2^14 p goes into the products, as in k_paged_few
+            const float mm = (F32 ? 0.0f : 14.0f) - (m == -INFINITY ? 0.0f : m);
+            half8 ph[2 * U], pl[F32 ? 2 * U : 1];
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int w = 0; w < VW; w++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) sp |= special_bits<F8>(cells[u][d * VW + w][c]);
-            if (__any(sp != 0)) {
-                if (lane == 0) map.note(st / (64 / KT) - pt.t0);
+                for (int r = 0; r < 16; r++) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, mm));
+                    l += e;
+                    if constexpr (F32) {
+                        half_t hi, lo;
+                        split16(e * 16384.0f, hi, lo);
+                        ph[2 * u + (r >> 3)][r & 7] = hi;
+                        pl[2 * u + (r >> 3)][r & 7] = lo;
+                    } else {
+                        ph[2 * u + (r >> 3)][r & 7] = (half_t)e;
+                    }
+                }
+            if (!full) {
+                // cells of tokens that do not exist are taken as 0
 #pragma unroll
                 for (int u = 0; u < U; u++)
 #pragma unroll
@@ -813,24 +797,49 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
 #pragma unroll
                         for (int w = 0; w < VW; w++)
 #pragma unroll
-                            for (int c = 0; c < 4; c++) cells[u][d * VW + w][c] = without_special<F8>(cells[u][d * VW + w][c]);
+                            for (int c = 0; c < 4; c++) {
+                                constexpr int PER = F8 ? 4 : 2;
+                                const int n = have[u] - PER * (4 * w + c);
+                                cells[u][d * VW + w][c] &= n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
+                            }
             }
+            if (careful) {
+                uint32_t sp = 0;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int c = 0; c < KW; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            sp |= special_bits<F8>(cells[u][c][e]);
+                            cells[u][c][e] = without_special<F8>(cells[u][c][e]);
+                        }
+                if (sp) map.note(st / (64 / KT) - pt.t0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        half8 v;
+                        if constexpr (F8)
+                            v = j ? f8_half8(cells[u][d * VW].z, cells[u][d * VW].w, vs[u]) : f8_half8(cells[u][d * VW].x, cells[u][d * VW].y, vs[u]);
+                        else
+                            v = __builtin_bit_cast(half8, cells[u][d * VW + j]);
+                        o[d] = mfma32(v, ph[2 * u + j], o[d]);
+                        if constexpr (F32) o[d] = mfma32(v, pl[2 * u + j], o[d]);
+                    }
+            if (st + 4 < s1) load_k(st + 4);
         }
+        if (careful) break;
+        bool odd = false;
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    half8 v;
-                    if constexpr (F8)
-                        v = j ? f8_half8(cells[u][d * VW].z, cells[u][d * VW].w, vs[u]) : f8_half8(cells[u][d * VW].x, cells[u][d * VW].y, vs[u]);
-                    else
-                        v = __builtin_bit_cast(half8, cells[u][d * VW + j]);
-                    o[d] = mfma32(v, ph[2 * u + j], o[d]);
-                    if constexpr (F32) o[d] = mfma32(v, pl[2 * u + j], o[d]);
-                }
-        if (st + 4 < s1) load_k(st + 4);
+            for (int r = 0; r < 16; r++) odd |= !(fabsf(o[d][r]) <= 3.402823466e38f);
+        if (!__any(odd)) break;
+        careful = true;
     }
 
     // ---- the four waves' results
@@ -864,7 +873,7 @@ template <int HD> struct many_lds {
     static constexpr int KS = 64 * 16 + 16;             // bytes per key chunk (the rest of a bank row: writes spread)
     static constexpr int VS = HD * 16 + 64;             // bytes per half block of values
     static constexpr int K = (HD / 8) * KS, V = 8 * VS;
-    static constexpr int FLAGS = 2 * 4 * 4 + (int)sizeof(special_map);   // per buffer: 4 counts of tokens
+    static constexpr int FLAGS = 12 * 4 + (int)sizeof(special_map);      // per buffer: 4 counts of tokens; one mark
     static constexpr int BYTES = 2 * (K + V) + FLAGS;
 };
 
@@ -881,8 +890,8 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
     constexpr int PER_BLOCK = UNITS / 4;
     using lds_t = many_lds<HD>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    int * flags = (int *)(lds + 2 * (lds_t::K + lds_t::V));      // [2][4]
-    special_map & map = *(special_map *)(flags + 8);
+    int * flags = (int *)(lds + 2 * (lds_t::K + lds_t::V));      // [2][4], the mark of a careful pass
+    special_map & map = *(special_map *)(flags + 12);
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
     const unit_at un = unit_of(blockIdx.x, p.Hkv, a.tiles);
     if (un.kvh >= p.Hkv) return;
@@ -900,6 +909,99 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
     const seen_t last = pg_seen(p0 + max(w1, 0) / a.G, keys, a.causal, a.window);
     const int f = min(w0 + i, f1), row = at.q.r0 + f / a.G, head = un.kvh * a.G + f % a.G;
     const seen_t me = pg_seen(p0 + f / a.G, keys, a.causal, a.window);
+
+    // ---- loader: this thread's 16-byte units of a tile.  A unit's block is the same for its whole wave, but
+    // its page and scales are held per lane (loads through the vector cache, counted with the cells', not
+    // scalar ones, which would be waited for with the LDS reads).
+    u32x4 kr[LU], vr[LU];
+    f32x2 scale[LU];
+    int page[LU], have[LU];
+    int zero;
+    asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+    const int32_t * const pages = p.pages + (int64_t)at.s * p.ld_pages + zero;
+    const int bs = p.page_shift - 4;                    // log2 of a page's blocks
+    const uint32_t page_units = (uint32_t)p.Hkv << bs;  // blocks of a page
+    // unit w: number `in` of block b0 + BW w
+    constexpr int BW = NT / PER_BLOCK;
+    static_assert(NT % PER_BLOCK == 0 && BW * LU == 4, "whole blocks");
+    const int b0 = __builtin_amdgcn_readfirstlane(tid / PER_BLOCK), in = tid % PER_BLOCK;
+    uint32_t lk, lv;                                    // where unit 0 goes in LDS; the others at k_step, v_step
+    {
+        constexpr int ROW = HD * CB / 16;               // units per token
+        const int tok = in / ROW, c = in % ROW;
+        const int slot = 32 * (b0 >> 1) + 8 * (tok >> 2) + 4 * (b0 & 1) + (tok & 3);
+        lk = (F8 ? 2 * c : c) * lds_t::KS + slot * 16;
+        lv = lds_t::K + (F8 ? 2 * b0 * lds_t::VS + in * 16 : (2 * b0 + (in & 1)) * lds_t::VS + (in >> 1) * 16);
+    }
+    auto k_step = [](int w) { return BW == 1 ? (32 * (w >> 1) + 4 * (w & 1)) * 16 : 32 * (BW / 2) * w * 16; };
+    auto v_step = [](int w) { return 2 * BW * w * lds_t::VS; };
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int w = 0; w < LU; w++) {
+            const int pos = 64 * t + 16 * (b0 + BW * w);
+            page[w] = -1;
+            if (t < pt.t1 && pos < p.cap) page[w] = pages[pos >> p.page_shift];
+        }
+    };
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int w = 0; w < LU; w++) {
+            const int b = b0 + BW * w;
+            const bool is = (uint32_t)page[w] < (uint32_t)p.n_pages;
+            // no page: page 0, not used
+            const uint64_t blk = (uint64_t)(is ? (uint32_t)page[w] : 0u) * page_units +
+                                 (uint32_t)((un.kvh << bs) + ((4 * t + b) & ((1 << bs) - 1)));
+            const uint64_t unit = blk * PER_BLOCK + in;
+            kr[w] = ((const u32x4 *)p.k)[unit];
+            vr[w] = ((const u32x4 *)p.v)[unit];
+            have[w] = is ? pg_clamp(keys - 64 * t - 16 * b, 0, 16) : 0;
+            if constexpr (F8) {
+                scale[w] = *(const f32x2 *)(p.scale + 2 * blk);
+                if (!is) scale[w] = f32x2{1.0f, 1.0f};
+            }
+        }
+        look_up(t + 1);
+    };
+    bool careful = false;
+    auto store = [&](int buf, int t) __attribute__((always_inline)) {
+        uint8_t * to = lds + buf * (lds_t::K + lds_t::V);
+#pragma unroll
+        for (int w = 0; w < LU; w++) {
+            if constexpr (F8) {
+                *(half8 *)(to + lk + k_step(w)) = f8_half8(kr[w].x, kr[w].y, scale[w].x);
+                *(half8 *)(to + lk + k_step(w) + lds_t::KS) = f8_half8(kr[w].z, kr[w].w, scale[w].x);
+            } else {
+                *(u32x4 *)(to + lk + k_step(w)) = kr[w];
+            }
+            // cells of tokens that do not exist are taken as 0
+            if (__any(have[w] < 16)) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    constexpr int PER = F8 ? 4 : 2;                          // tokens per word
+                    const int n = have[w] - PER * (4 * (F8 ? 0 : in & 1) + k);
+                    vr[w][k] &= n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
+                }
+            }
+            if (careful) {
+                uint32_t sp = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    sp |= special_bits<F8>(vr[w][k]);
+                    vr[w][k] = without_special<F8>(vr[w][k]);
+                }
+                if (sp) map.note(t - pt.t0);
+            }
+            if constexpr (F8) {
+                *(half8 *)(to + lv + v_step(w)) = f8_half8(vr[w].x, vr[w].y, scale[w].y);
+                *(half8 *)(to + lv + v_step(w) + lds_t::VS) = f8_half8(vr[w].z, vr[w].w, scale[w].y);
+            } else {
+                *(u32x4 *)(to + lv + v_step(w)) = vr[w];
+            }
+            if (in == 0) flags[4 * buf + b0 + BW * w] = have[w];
+        }
+    };
+
+    look_up(pt.t0);                                     // on its way with Q
 
     half8 qh[QS], ql[F32 ? QS : 1];
     float sc = LOG2E_F / sqrtf((float)HD);
@@ -936,211 +1038,158 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
         }
     }
 
-    // Q is waited for here, not by the loop's first products (whose wait would be for the loads of the
-    // next tile in every later turn)
-#pragma unroll
-    for (int c = 0; c < QS; c++) {
-        asm volatile("" : "+v"(qh[c]));
-        if constexpr (F32) asm volatile("" : "+v"(ql[c]));
-    }
-
-    // ---- loader: this thread's 16-byte units of a tile; a unit's block is the same for its whole wave.
-    // Pages are looked up a tile ahead: lane 2b + side (mod 8) holds the page of block b and, with the
-    // cells, loads its scale of that side.
-    u32x4 kr[LU], vr[LU];
-    int have[LU], page = -1;
-    float scale = 1.0f;
-    auto look_up = [&](int t) __attribute__((always_inline)) {
-        const int pos = 64 * t + 16 * ((lane >> 1) & 3);
-        page = -1;
-        if (t < pt.t1 && pos < p.cap) page = p.pages[(int64_t)at.s * p.ld_pages + (pos >> p.page_shift)];
-        if (page >= p.n_pages) page = -1;
+    // ---- one tile's steps
+    auto read_k = [&](int buf, int c, int u) __attribute__((always_inline)) {
+        return *(const half8 *)(lds + buf * (lds_t::K + lds_t::V) + (2 * c + h) * lds_t::KS + (32 * u + i) * 16);
     };
-    const int bs = p.page_shift - 4;                    // log2 of a page's blocks
-    auto load = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-        for (int w = 0; w < LU; w++) {
-            const int u = tid + NT * w, b = (64 * wv + NT * w) / PER_BLOCK, in = u % PER_BLOCK;
-            const int pg = __builtin_amdgcn_readlane(page, 2 * b);
-            // no page: block 0 of the cache, not used
-            const int64_t blk = pg < 0 ? 0 : (((int64_t)pg * p.Hkv + un.kvh) << bs) + ((4 * t + b) & ((1 << bs) - 1));
-            kr[w] = ((const u32x4 *)p.k)[blk * PER_BLOCK + in];
-            vr[w] = ((const u32x4 *)p.v)[blk * PER_BLOCK + in];
-            have[w] = pg < 0 ? 0 : pg_clamp(keys - 64 * t - 16 * b, 0, 16);
-        }
-        if constexpr (F8) {
-            const int64_t blk = (((int64_t)max(page, 0) * p.Hkv + un.kvh) << bs) + ((4 * t + ((lane >> 1) & 3)) & ((1 << bs) - 1));
-            scale = p.scale[2 * blk + (lane & 1)];
-            scale = page < 0 ? 1.0f : scale;
-        }
-        look_up(t + 1);
+    auto read_v = [&](int buf, int d, int g) __attribute__((always_inline)) {   // (u, half of the block) = (g / 2, g % 2)
+        return *(const half8 *)(lds + buf * (lds_t::K + lds_t::V) + lds_t::K + (2 * (2 * (g >> 1) + h) + (g & 1)) * lds_t::VS +
+                                (32 * d + i) * 16);
     };
-    auto store = [&](int buf, int t) __attribute__((always_inline)) {
-        uint8_t * kl = lds + buf * (lds_t::K + lds_t::V), * vl = kl + lds_t::K;
-#pragma unroll
-        for (int w = 0; w < LU; w++) {
-            const int u = tid + NT * w, b = (64 * wv + NT * w) / PER_BLOCK, in = u % PER_BLOCK;
-            // keys: token and 16 bytes of its row -> row of S^T tile, chunks
-            constexpr int ROW = HD * CB / 16;                                // units per token
-            const int tok = in / ROW, c = in % ROW;
-            const int slot = 32 * (b >> 1) + 8 * (tok >> 2) + 4 * (b & 1) + (tok & 3);
-            const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 2 * b));
-            const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 2 * b + 1));
-            if constexpr (F8) {
-                *(half8 *)(kl + (2 * c) * lds_t::KS + slot * 16) = f8_half8(kr[w].x, kr[w].y, ks);
-                *(half8 *)(kl + (2 * c + 1) * lds_t::KS + slot * 16) = f8_half8(kr[w].z, kr[w].w, ks);
-            } else {
-                *(u32x4 *)(kl + c * lds_t::KS + slot * 16) = kr[w];
-            }
-            // values: cells of tokens that do not exist are taken as 0
-            if (have[w] < 16) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    constexpr int PER = F8 ? 4 : 2;                          // tokens per word
-                    const int n = have[w] - PER * (4 * (F8 ? 0 : in & 1) + k);
-                    vr[w][k] &= n >= PER ? 0xffffffffu : n <= 0 ? 0u : (1u << (n * (32 / PER))) - 1u;
-                }
-            }
-            uint32_t sp = 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) sp |= special_bits<F8>(vr[w][k]);
-            if (sp) {
-                map.note(t - pt.t0);
-#pragma unroll
-                for (int k = 0; k < 4; k++) vr[w][k] = without_special<F8>(vr[w][k]);
-            }
-            if constexpr (F8) {
-                *(half8 *)(vl + (2 * b) * lds_t::VS + in * 16) = f8_half8(vr[w].x, vr[w].y, vs);
-                *(half8 *)(vl + (2 * b + 1) * lds_t::VS + in * 16) = f8_half8(vr[w].z, vr[w].w, vs);
-            } else {
-                *(u32x4 *)(vl + (2 * b + (in & 1)) * lds_t::VS + (in >> 1) * 16) = vr[w];
-            }
-            if (in == 0) flags[4 * buf + b] = have[w];
-        }
-    };
-
-    float m = -INFINITY, l = 0.0f;
+    // operands read ahead of their products: fewer where f32 results and f16 cells need the registers
+    constexpr int KH = QS / (F32 && !F8 ? 4 : 2), VH = DT / (F32 && !F8 && DT == 4 ? 4 : 2);
+    float m, l;
     float16v o[DT];
+    half8 ph[4], pl[F32 ? 4 : 1];
+    auto mask = [&](float16v (&s)[2], int buf, int t) __attribute__((always_inline)) {
+        const int4 there = *(const int4 *)(flags + 4 * buf);
+        if (64 * t >= last.lo && 64 * t + 63 <= first.hi && min(min(there.x, there.y), min(there.z, there.w)) == 16) return;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+        for (int u = 0; u < 2; u++) {
+            const int k0 = 64 * t + 32 * u + 16 * h;
+            const int n = u == 0 ? (h ? there.y : there.x) : (h ? there.w : there.z);
+            const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, n), 0, 16);
 #pragma unroll
-        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+            for (int r = 0; r < 16; r++) s[u][r] = r >= lo && r < hi ? s[u][r] : -INFINITY;
+        }
+    };
+    // Probabilities against the running maximum as it is (weigh); where a lane's sum of them says that one
+    // may leave f16's range, or a query has no maximum yet, the maximum is taken anew and the sums are
+    // brought to it (settle).  2^6 p (f32 results: 2^7 p, applied after the exponential) goes into the
+    // products: small probabilities keep their bits.
+    auto weigh = [&](const float16v (&s)[2], int u, int r, float mm) __attribute__((always_inline)) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, mm));
+        if constexpr (F32) {
+            half_t hi, lo;
+            split16(e * 128.0f, hi, lo);
+            ph[2 * u + (r >> 3)][r & 7] = hi;
+            pl[2 * u + (r >> 3)][r & 7] = lo;
+        } else {
+            ph[2 * u + (r >> 3)][r & 7] = (half_t)e;
+        }
+        return e;
+    };
+    auto reference = [&]() __attribute__((always_inline)) { return (F32 ? 0.0f : 6.0f) - (m == -INFINITY ? 0.0f : m); };
+    auto settle = [&](const float16v (&s)[2], float sum) __attribute__((always_inline)) {
+        if (__any(m == -INFINITY || sum > (F32 ? 256.0f : 16384.0f))) {
+            float tm = s[0][0];
+#pragma unroll
+            for (int r = 0; r < 16; r++) tm = fmaxf(tm, fmaxf(s[0][r], s[1][r]));
+            tm = half_max(tm) * sc;
+            const float to = fmaxf(m, tm), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= f;
+            m = to;
+            sum = 0.0f;
+            const float mm = reference();
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) sum += weigh(s, u, r, mm);
+        }
+        l += sum;
+    };
 
     if (tid < MAP_BITS / 32) map.w[tid] = 0;
-    __syncthreads();
-    if (pt.t0 < pt.t1) {
-        look_up(pt.t0);
+    if (tid == 0) flags[8] = 0;
+    while (true) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+        __syncthreads();
+        // In registers: tile t + 1, loaded in the turn before; it goes to LDS as turn t begins, and the next
+        // one is loaded.  Tiles behind the last are read as no page and not used.
         load(pt.t0);
         store(0, pt.t0);
-    }
-    __syncthreads();
-    for (int t = pt.t0; t < pt.t1; t++) {
-        const int buf = (t - pt.t0) & 1;
-        if (t + 1 < pt.t1) load(t + 1);
-        if (!idle && 64 * t <= last.hi && 64 * t + 63 >= first.lo) {
-            const uint8_t * kl = lds + buf * (lds_t::K + lds_t::V), * vl = kl + lds_t::K;
-            // operands are read ahead of the products that take them, HALF of a side at a time with f32
-            // results (registers)
-            constexpr int KH = QS / 2;
-            float16v s[2];
+        load(pt.t0 + 1);
+        // Q is waited for here, not by the loop's first products (whose wait would be for the loads of the
+        // next tile in every later turn)
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
+        for (int c = 0; c < QS; c++) {
+            asm volatile("" : "+v"(qh[c]));
+            if constexpr (F32) asm volatile("" : "+v"(ql[c]));
+        }
+        __syncthreads();
+        for (int t = pt.t0; t < pt.t1; t++) {
+            const int buf = (t - pt.t0) & 1;
+            store(buf ^ 1, t + 1);
+            load(t + 2);
+            if (!idle && 64 * t <= last.hi && 64 * t + 63 >= first.lo) {
+                float16v s[2];
 #pragma unroll
-            for (int c0 = 0; c0 < QS; c0 += KH) {
-                half8 kf[KH][2];
+                for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < KH; c++)
+                for (int c0 = 0; c0 < QS; c0 += KH) {
+                    half8 kf[KH][2];
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
-                        kf[c][u] = *(const half8 *)(kl + (2 * (c0 + c) + h) * lds_t::KS + (32 * u + i) * 16);
-                __builtin_amdgcn_sched_barrier(0);
+                    for (int c = 0; c < KH; c++)
 #pragma unroll
-                for (int c = 0; c < KH; c++)
+                        for (int u = 0; u < 2; u++) kf[c][u] = read_k(buf, c0 + c, u);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        s[u] = mfma32(kf[c][u], qh[c0 + c], s[u]);
-                        if constexpr (F32) s[u] = mfma32(kf[c][u], ql[c0 + c], s[u]);
-                    }
-            }
-            constexpr int VH = DT / 2;
-            half8 vf[VH][4];
-            auto read_v = [&](int d0) __attribute__((always_inline)) {
+                    for (int c = 0; c < KH; c++)
 #pragma unroll
-                for (int d = 0; d < VH; d++)
-#pragma unroll
-                    for (int g = 0; g < 4; g++)                              // (u, half) = (g / 2, g % 2)
-                        vf[d][g] = *(const half8 *)(vl + (2 * (2 * (g >> 1) + h) + (g & 1)) * lds_t::VS + (32 * (d0 + d) + i) * 16);
-            };
-            const int4 there = *(const int4 *)(flags + 4 * buf);
-            const bool full = 64 * t >= last.lo && 64 * t + 63 <= first.hi &&
-                              min(min(there.x, there.y), min(there.z, there.w)) == 16;
-            if (!full) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int k0 = 64 * t + 32 * u + 16 * h;
-                    const int n = u == 0 ? (h ? there.y : there.x) : (h ? there.w : there.z);
-                    const int lo = pg_clamp(me.lo - k0, 0, 16), hi = pg_clamp(min(me.hi + 1 - k0, n), 0, 16);
-#pragma unroll
-                    for (int r = 0; r < 16; r++) s[u][r] = r >= lo && r < hi ? s[u][r] : -INFINITY;
+                        for (int u = 0; u < 2; u++) {
+                            s[u] = mfma32(kf[c][u], qh[c0 + c], s[u]);
+                            if constexpr (F32) s[u] = mfma32(kf[c][u], ql[c0 + c], s[u]);
+                        }
                 }
-            }
-            // Probabilities against the running maximum as it is; where a lane's sum of them says that one
-            // may leave f16's range, or a query has no maximum yet, the maximum is taken anew and the
-            // sums are brought to it.  2^6 p (f32 results: 2^7 p, applied after the exponential) goes
-            // into the products: small probabilities keep their bits.
-            half8 ph[4], pl[F32 ? 4 : 1];
-            auto weigh = [&]() __attribute__((always_inline)) {
-                const float mm = (F32 ? 0.0f : 6.0f) - (m == -INFINITY ? 0.0f : m);
+                mask(s, buf, t);
+                const float mm = reference();
                 float sum = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, mm));
-                        sum += e;
-                        if constexpr (F32) {
-                            half_t hi, lo;
-                            split16(e * 128.0f, hi, lo);
-                            ph[2 * u + (r >> 3)][r & 7] = hi;
-                            pl[2 * u + (r >> 3)][r & 7] = lo;
-                        } else {
-                            ph[2 * u + (r >> 3)][r & 7] = (half_t)e;
+                    for (int r = 0; r < 16; r++) sum += weigh(s, u, r, mm);
+                settle(s, sum);
+#pragma unroll
+                for (int d0 = 0; d0 < DT; d0 += VH) {
+                    half8 vf[VH][4];
+#pragma unroll
+                    for (int d = 0; d < VH; d++)
+#pragma unroll
+                        for (int g = 0; g < 4; g++) vf[d][g] = read_v(buf, d0 + d, g);
+#pragma unroll
+                    for (int g = 0; g < 4; g++)
+#pragma unroll
+                        for (int d = 0; d < VH; d++) {
+                            o[d0 + d] = mfma32(vf[d][g], ph[g], o[d0 + d]);
+                            if constexpr (F32) o[d0 + d] = mfma32(vf[d][g], pl[g], o[d0 + d]);
                         }
-                    }
-                return sum;
-            };
-            float sum = weigh();
-            if (__any(m == -INFINITY || sum > (F32 ? 256.0f : 16384.0f))) {
-                float tm = s[0][0];
-#pragma unroll
-                for (int r = 0; r < 16; r++) tm = fmaxf(tm, fmaxf(s[0][r], s[1][r]));
-                tm = half_max(tm) * sc;
-                const float to = fmaxf(m, tm), r = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-                l *= r;
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] *= r;
-                m = to;
-                sum = weigh();
+                }
             }
-            l += sum;
-#pragma unroll
-            for (int d0 = 0; d0 < DT; d0 += VH) {
-                read_v(d0);
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-#pragma unroll
-                    for (int d = 0; d < VH; d++) {
-                        o[d0 + d] = mfma32(vf[d][g], ph[g], o[d0 + d]);
-                        if constexpr (F32) o[d0 + d] = mfma32(vf[d][g], pl[g], o[d0 + d]);
-                    }
-            }
+            __syncthreads();
         }
-        if (t + 1 < pt.t1) store(buf ^ 1, t + 1);
+        if (careful) break;
+        // a sum that is not finite: there is such a value among the cells, or such a score
+        bool odd = false;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) odd |= !(fabsf(o[d][r]) <= 3.402823466e38f);
+        if (!idle && __any(odd) && lane == 0) flags[8] = 1;
         __syncthreads();
+        if (!flags[8]) break;
+        careful = true;
+        look_up(pt.t0);
     }
 
-    if (map.any()) {
-        // every wave is past the tiles (the barrier above): their room takes the sums, 32 dims at a time
+    if (careful && map.any()) {
+        // every wave is past the tiles (the barriers above): their room takes the sums, 32 dims at a time
         constexpr int OS = 34;
         static_assert(T * OS * 4 <= 2 * (lds_t::K + lds_t::V), "room for the sums");
         float * so = (float *)lds + (32 * wv + i) * OS;
