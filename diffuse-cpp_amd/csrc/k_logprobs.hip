@@ -2,19 +2,20 @@
 //
 //   m = max x,  S = sum e,  T = sum e (x - m),  e = exp(x - m)
 //   log p_t = (x_t - m) - log S,   entropy = log S - T / S
-// A row is cut into pieces of 64 * 4 * U logits, one wave each, so that one row fills the chip as
+// A row is cut into pieces of LP_PIECE logits, one wave each, so that one row fills the chip as
 // well as many do.  A wave keeps its piece in registers: one read gives m, S, T and the piece's
 // candidates for the alternatives; no barrier, nothing shared.  A second kernel joins a row's pieces.
 //
 // Alternatives: of the 128 values that are the two largest of each lane, the n-th largest is a bound
 // that at least n elements of the piece reach; few more do (a third one of a lane, equal values).
-// It is found bit by bit, counting with ballots, and what reaches it is listed.  A piece where too
-// many do (equal values) finds its n largest one after another instead.
+// It is found by halving, counting with ballots, and what reaches it is listed.  A piece where too many
+// do (equal values) finds the n-th largest of all its elements the same way.
 #include "dfx_device.h"
 
 #include <algorithm>
 
 #define LP_MAX_TOP 64
+#define LP_PIECE 2048   // logits of a wave: 32 registers a lane (1024: one row with 5 alternatives no faster, 64 rows 6 % slower)
 #define LOG2E_F 1.44269504088896341f
 
 // A candidate as one integer whose order is that of the alternatives: the value in the high word
@@ -34,16 +35,30 @@ __device__ __forceinline__ int lp_index(uint64_t c) { return (int)~(uint32_t)c; 
 
 struct lp_part { float m, S, T, pad; };
 
-// A bound that at least n of the wave's 128 keys reach: exactly n if no two are equal there.
+// A bound that at least n <= 64 of the wave's 128 keys (a >= b in each lane) reach, and, but for equal
+// ones, at most n + LP_SLACK: between the least and the largest a, halved until the count is near.
+#define LP_SLACK 6
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));
+    return max(max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
 __device__ __forceinline__ uint32_t wave_bound(uint32_t a, uint32_t b, int n) {
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t c = t | (1u << bit);
-        const int k = __popcll(__ballot(a >= c)) + __popcll(__ballot(b >= c));
-        if (k >= n) t = c;
-        if (k == n) break;
+    uint32_t lo = ~wave_max_u(~a), hi = wave_max_u(a);              // all 64 a reach lo (0: lanes with nothing)
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        const int k = __popcll(__ballot(a >= mid)) + __popcll(__ballot(b >= mid));
+        if (k < n) {
+            hi = mid - 1;
+            continue;
+        }
+        lo = mid;
+        if (k <= n + LP_SLACK) break;
     }
-    return t;
+    return lo;
 }
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     for (int o = 32; o > 0; o >>= 1) {
@@ -53,7 +68,7 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     return v;
 }
 
-template <int U, bool VEC>
+template <bool VEC>
 __global__ void __launch_bounds__(256, 4) k_lp_pieces(const float * __restrict__ logits, int64_t ld, int64_t n_logits,
                                                       const int32_t * __restrict__ rows, int V, int pieces, int n_top,
                                                       int cap, lp_part * __restrict__ part,
@@ -64,7 +79,8 @@ __global__ void __launch_bounds__(256, 4) k_lp_pieces(const float * __restrict__
     const int64_t row = rows ? (int64_t)rows[blockIdx.y] : (int64_t)blockIdx.y;
     if (row < 0 || row >= n_logits) return;
     const float * x = logits + row * ld;
-    const int base = piece * (256 * U);
+    constexpr int U = LP_PIECE / 256;
+    const int base = piece * LP_PIECE;
     // element e = 4 u + c of the lane
     auto index = [&](int e) { return base + (VEC ? 256 * (e >> 2) + 4 * lane + (e & 3) : 64 * e + lane); };
     float v[4 * U];
@@ -129,21 +145,53 @@ __global__ void __launch_bounds__(256, 4) k_lp_pieces(const float * __restrict__
         if (n > cap) break;
     }
     if (n > cap) {
-        // too many equal values: the n_top best, each the best below the one before
-        uint64_t last = ~0ull;
-        for (n = 0; n < n_top; n++) {
-            uint64_t best = 0;
-#pragma unroll 1
-            for (int e = 0; e < 4 * U; e++) {
-                const int i = index(e);
-                const uint64_t c = i < V ? lp_cand(lp_key(x[i]), i) : 0;
-                if (c < last && c > best) best = c;
-            }
-            best = wave_max_u64(best);
-            if ((uint32_t)(best >> 32) < LP_LOWEST) break;
-            if (lane == 0) out[n] = best;
-            last = best;
+        // Too many, equal ones among them: the bound is taken exactly (the n_top-th largest of the piece's
+        // elements, counting them all), what is above it listed, and of those that equal it the first.
+        auto count = [&](uint32_t key) __attribute__((always_inline)) {
+            const float f = lp_value(key);
+            int k = 0;
+#pragma unroll
+            for (int e = 0; e < 4 * U; e++) k += __popcll(__ballot(v[e] >= f));
+            return k;
+        };
+        uint32_t lo = bound, hi = wave_max_u(lp_key(m1));
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            if (count(mid) >= n_top) lo = mid;
+            else hi = mid - 1;
         }
+        const float at_f = lp_value(lo), above_f = lp_value(lo + 1);  // behind +inf: NaN, nothing is above
+        const uint64_t lower = (1ull << lane) - 1;
+        int above = 0, equal = count(lo + 1);                         // places of the next of either
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int mine = equal;                                         // index order: lane by lane (VEC), or element by element
+            if constexpr (VEC)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint64_t eq = __ballot(v[4 * u + c] >= at_f && !(v[4 * u + c] >= above_f));
+                    mine += __popcll(eq & lower);
+                    equal += __popcll(eq);
+                }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int e = 4 * u + c;
+                const bool gt = v[e] >= above_f, eq = v[e] >= at_f && !gt;
+                const uint64_t has = __ballot(gt);
+                if (gt) out[above + __popcll(has & lower)] = lp_cand(lp_key(v[e]), index(e));
+                above += __popcll(has);
+                if constexpr (VEC) {
+                    if (eq && mine < n_top) out[mine] = lp_cand(lp_key(v[e]), index(e));
+                    mine += eq;
+                } else {
+                    const uint64_t he = __ballot(eq);
+                    const int at = equal + __popcll(he & lower);
+                    if (eq && at < n_top) out[at] = lp_cand(lp_key(v[e]), index(e));
+                    equal += __popcll(he);
+                }
+            }
+        }
+        n = n_top;
     }
     for (int j = n + lane; j < cap; j += 64) out[j] = 0;
 }
@@ -151,6 +199,7 @@ __global__ void __launch_bounds__(256, 4) k_lp_pieces(const float * __restrict__
 // One workgroup per row: sums of the pieces in double, then the n_top best of the pieces' candidates
 // the same way: a bound from each lane's two largest, what reaches it into LDS, places by counting.
 #define LP_LIST 2048
+#define LP_MANY 128
 #define LP_JOIN 1024
 __global__ void __launch_bounds__(LP_JOIN) k_lp_join(const float * __restrict__ logits, int64_t ld, int64_t n_logits,
                                                      const int32_t * __restrict__ rows, int V, int pieces, int n_top,
@@ -274,6 +323,30 @@ __global__ void __launch_bounds__(LP_JOIN) k_lp_join(const float * __restrict__ 
         top_logprob[r * n_top + at] = (float)(((double)value - (double)m) - log_s);
     };
     int n = list_n;
+    if (n > LP_MANY && n <= LP_LIST) {
+        // more than are quickly counted: one wave takes their bound, and keeps what reaches it
+        __syncthreads();                               // list_n has been read
+        if (wv == 0) {
+            k1 = k2 = 0;
+            for (int j = lane; j < n; j += 64) {
+                const uint32_t k = (uint32_t)(list[j] >> 32);
+                k2 = max(k2, min(k1, k));
+                k1 = max(k1, k);
+            }
+            bound = wave_bound(k1, k2, n_top);
+            int kept = 0;
+            for (int j0 = 0; j0 < n; j0 += 64) {       // places before the ones that are read next
+                const uint64_t c = j0 + lane < n ? list[j0 + lane] : 0;
+                const bool is = c && (uint32_t)(c >> 32) >= bound;
+                const uint64_t has = __ballot(is);
+                if (is) list[kept + __popcll(has & ((1ull << lane) - 1))] = c;
+                kept += __popcll(has);
+            }
+            if (lane == 0) list_n = kept;
+        }
+        __syncthreads();
+        n = list_n;
+    }
     if (n <= LP_LIST) {
         for (int e = tid; e < n; e += nt) {
             const uint64_t c = list[e];
@@ -320,12 +393,13 @@ __global__ void __launch_bounds__(LP_JOIN) k_lp_join(const float * __restrict__ 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-struct lp_plan { int u, pieces, cap; size_t part_bytes, bytes; };
+struct lp_plan { int pieces, cap; size_t part_bytes, bytes; };
 static lp_plan lp_plan_of(int64_t n_rows, int64_t V, int n_top) {
     lp_plan p;
-    p.u = n_rows * ((V + 4095) / 4096) >= 4096 ? 8 : 4;
-    p.pieces = (int)((V + 256 * p.u - 1) / (256 * p.u));
-    p.cap = n_top > 0 ? n_top + 12 : 0;
+    p.pieces = (int)((V + LP_PIECE - 1) / LP_PIECE);
+    // n_top, the bound's slack, and the elements that are third or later in their lane: few but for large
+    // n_top (64 of 2048: about 10)
+    p.cap = n_top > 0 ? n_top + 12 + n_top * n_top / 100 : 0;
     p.part_bytes = align256((size_t)n_rows * p.pieces * sizeof(lp_part));
     p.bytes = p.part_bytes + (size_t)n_rows * p.pieces * p.cap * sizeof(uint64_t);
     return p;
@@ -368,22 +442,18 @@ extern "C" int dfx_token_logprobs(const float * logits, int64_t ld, int64_t n_lo
         const int32_t * rw = rows ? rows + r0 : nullptr;
         lp_part * pp = part + r0 * p.pieces;
         uint64_t * cc = cand + r0 * p.pieces * p.cap;
-#define PIECES(U, VEC)                                                                                                \
-    hipLaunchKernelGGL((k_lp_pieces<U, VEC>), grid, dim3(256), 0, st, lg, ld, nl, rw, (int)V, p.pieces, n_top, p.cap,  \
+#define PIECES(VEC)                                                                                                   \
+    hipLaunchKernelGGL((k_lp_pieces<VEC>), grid, dim3(256), 0, st, lg, ld, nl, rw, (int)V, p.pieces, n_top, p.cap,  \
                        pp, cc)
-        if (p.u == 8) {
-            if (vec) PIECES(8, true);
-            else PIECES(8, false);
-        } else {
-            if (vec) PIECES(4, true);
-            else PIECES(4, false);
-        }
+        if (vec) PIECES(true);
+        else PIECES(false);
 #undef PIECES
         DFX_CHECK_LAUNCH("dfx_token_logprobs");
     }
-    // Threads of a row's join: a wave where there are no candidates; with them, one row takes 16 waves
-    // (8 candidates a thread, one round of loads), many rows 4.
-    const int waves = n_top == 0 ? 1 : n_rows <= 128 ? LP_JOIN / 64 : 4;
+    // Threads of a row's join: a wave where there are no candidates; with them, few rows take 16 waves
+    // (8 candidates a thread, one round of loads), more rows 8 and 4 (256 rows of 62 pieces, 20 alternatives:
+    // 39.8 us with 16 waves, 37.6 with 8, 37.9 with 4).
+    const int waves = n_top == 0 ? 1 : n_rows <= 128 ? LP_JOIN / 64 : n_rows <= 512 ? 8 : 4;
     hipLaunchKernelGGL(k_lp_join, dim3((unsigned)n_rows), dim3(64 * waves), 0, st, logits, ld, n_logits, rows, (int)V, p.pieces,
                        n_top, p.cap, part, cand, tokens, n_tok, logprob, entropy, top_id, top_logprob);
     DFX_CHECK_LAUNCH("dfx_token_logprobs (join)");

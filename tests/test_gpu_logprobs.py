@@ -142,6 +142,24 @@ def test_equal_masked_and_special_logits(gpu, V, top):
         check(run(x, tokens=tokens, top=top), x, tokens=tokens, top=top)
 
 
+@pytest.mark.parametrize("V", [1500, 126464, 126465])
+@pytest.mark.parametrize("top", [20, 64])
+def test_best_logits_side_by_side(gpu, V, top):
+    """The largest logits as neighbours, every fourth, 64 apart and 256 apart (one lane's elements), and runs of
+    equal values across lanes: the same order, the lowest index first."""
+    rng = np.random.default_rng(V + top)
+    x = rng.standard_normal((8, V)).astype(np.float32)
+    for r, step in enumerate((1, 2, 4, 64, 256)):
+        at = 7 + step * np.arange(min(80, (V - 8) // step))
+        x[r, at] = 20 + rng.standard_normal(len(at)).astype(np.float32)
+    x[5, 100:1000] = 9.0
+    x[6, 5::3] = 4.0
+    x[7, V // 2:] = np.float32(np.finfo(np.float32).min)
+    x[7, :V // 2] = np.where(rng.random(V // 2) < 30.0 / V, x[7, :V // 2], np.float32(np.finfo(np.float32).min))
+    tokens = rng.integers(0, V, (8, 1))
+    check(run(x, tokens=tokens, top=top), x, tokens=tokens, top=top)
+
+
 def test_ids_and_values_against_row_stats(gpu):
     """The best alternative and the entropy are those of dfx_row_stats on the same rows."""
     rng = np.random.default_rng(4)
