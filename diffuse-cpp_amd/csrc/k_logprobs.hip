@@ -405,7 +405,7 @@ static lp_plan lp_plan_of(int64_t n_rows, int64_t V, int n_top) {
     return p;
 }
 static bool lp_shape_ok(int64_t n_rows, int64_t V, int n_top) {
-    return n_rows >= 0 && n_rows <= (1 << 24) && V > 0 && V <= (1 << 30) && n_top >= 0 && n_top <= LP_MAX_TOP;
+    return n_rows >= 0 && n_rows <= (1 << 22) && V > 0 && V <= (1 << 30) && n_top >= 0 && n_top <= LP_MAX_TOP;
 }
 
 extern "C" size_t dfx_token_logprobs_ws_bytes(int64_t n_rows, int64_t V, int n_top) {

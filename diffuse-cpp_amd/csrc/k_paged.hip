@@ -366,6 +366,9 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES, 3) k_paged_append(paged_t p
 // ---------------------------------------------------------------------------
 static bool aligned(const void * ptr, uintptr_t to) { return ((uintptr_t)ptr & (to - 1)) == 0; }
 
+// Rows times heads of one call: what a grid of 256-thread workgroups holds in one dimension, halved.
+#define MAX_ROW_HEADS (1 << 23)
+
 // The kernel form of a cache and a batch; a status and message where they are not sound.
 int paged_of(const char * who, const dfx_paged_cache * c, const dfx_paged_batch * b, int n_head, paged_t * out) {
     if (!c || !b) {
@@ -396,9 +399,9 @@ int paged_of(const char * who, const dfx_paged_cache * c, const dfx_paged_batch 
         dfx_set_error("%s: cache buffers missing or not aligned (k, v: 16 bytes; scale: 8)", who);
         return DFX_ERR_ARG;
     }
-    if (b->n_seqs < 0 || b->n_rows < 0 || b->max_keys < 0 || (int64_t)b->n_rows * n_head > (1 << 29)) {
-        dfx_set_error("%s: bad batch seqs=%d rows=%d max_keys=%lld H=%d", who, b->n_seqs, b->n_rows,
-                      (long long)b->max_keys, n_head);
+    if (b->n_seqs < 0 || b->n_rows < 0 || b->max_keys < 0 || (int64_t)b->n_rows * n_head > MAX_ROW_HEADS) {
+        dfx_set_error("%s: bad batch seqs=%d rows=%d max_keys=%lld H=%d (rows times heads: at most %d)", who, b->n_seqs,
+                      b->n_rows, (long long)b->max_keys, n_head, MAX_ROW_HEADS);
         return DFX_ERR_ARG;
     }
     if (b->n_seqs > 0 && b->n_rows > 0 && (!b->rows || !b->n_keys || !b->pages || b->ld_pages <= 0)) {

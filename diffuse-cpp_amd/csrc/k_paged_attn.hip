@@ -600,8 +600,8 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
     const tile_at at = wave_tile_by_work<MID_T>(p, a.G, a.causal, a.window, un.tile);
     if (at.s < 0) return;
     const int nq = at.q.n * a.G, f0 = at.tile * MID_T, f1 = min(f0 + MID_T, nq) - 1;
-    const part_at pt = part_of(pg_tiles(at.q, f0, f1, a.G, a.causal, a.window), blockIdx.y, a.chunk, a.parts);
-    if ((int)blockIdx.y >= pt.parts) return;
+    const tiles_t all = pg_tiles(at.q, f0, f1, a.G, a.causal, a.window);
+    const part_at pt = {all.t0, all.t1, 1};
     const int keys = at.q.keys, p0 = keys - at.q.n;
     const int all_lo = pg_seen(p0 + f1 / a.G, keys, a.causal, a.window).lo;
     const int all_hi = pg_seen(p0 + f0 / a.G, keys, a.causal, a.window).hi;
@@ -899,8 +899,7 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
     if (at.s < 0) return;
     const int nq = at.q.n * a.G;
     const int f0 = at.tile * T, f1 = min(f0 + T, nq) - 1;
-    const part_at pt = part_of(pg_tiles(at.q, f0, f1, a.G, a.causal, a.window), blockIdx.y, a.chunk, a.parts);
-    if ((int)blockIdx.y >= pt.parts) return;
+    const tiles_t pt = pg_tiles(at.q, f0, f1, a.G, a.causal, a.window);
     const int keys = at.q.keys, p0 = keys - at.q.n;
     // this wave's queries, the keys that all and that any of them see
     const int w0 = f0 + 32 * wv, w1 = min(w0 + 31, f1);
@@ -1211,26 +1210,16 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
     if (idle || w0 + i > f1) return;
     l = half_sum(l);
     const int64_t rh = (int64_t)row * a.H + head;
-    float mul = F32 ? 1.0f / 128.0f : 1.0f;
-    if (pt.parts == 1) mul = l == 0.0f ? 0.0f : mul / l;
-    const int64_t at_part = (int64_t)blockIdx.y * p.n_rows * a.H + rh;
+    const float mul = l == 0.0f ? 0.0f : (F32 ? 1.0f / 128.0f : 1.0f) / l;
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             const int dim = 32 * d + 8 * b + 4 * h;
             const float4v v = {o[d][4 * b] * mul, o[d][4 * b + 1] * mul, o[d][4 * b + 2] * mul, o[d][4 * b + 3] * mul};
-            if (pt.parts > 1) *(float4v *)(a.part_o + at_part * HD + dim) = v;
-            else if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + dim) = v;
+            if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + dim) = v;
             else *(half4 *)((half_t *)a.out + rh * HD + dim) = half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
         }
-    if (a.parts > 1 && h == 0) {
-        if (blockIdx.y == 0) a.n_parts[rh] = pt.parts;
-        if (pt.parts > 1) {
-            a.part_ml[2 * at_part] = m;
-            a.part_ml[2 * at_part + 1] = l;
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1328,7 +1317,8 @@ static attn_plan plan_of(const paged_t & p, int H, int64_t max_keys, int window,
     r.T = queries <= 16 * seqs || all <= 512 * 16 ? FEW_T : queries <= 32 * seqs || all <= 1024 * 32 ? MID_T : MANY_T;
     r.tiles = (int)(queries / r.T + seqs);
     const int64_t units = (int64_t)p.Hkv * std::max<int64_t>(seqs, queries / r.T);
-    const int64_t want = std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, 512 / units));
+    // 32 and 128 queries come in more than 256 workgroups (8192 / 32, 32768 / 128): their ranges stay whole
+    const int64_t want = r.T == FEW_T ? std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, 512 / units)) : 1;
     // key tiles that a query tile can see
     int64_t kt = (std::min<int64_t>(std::max<int64_t>(max_keys, 1), p.cap) + 63) / 64;
     r.most = kt <= WHOLE ? 1 : (int)std::min<int64_t>(want, (kt + MIN_CHUNK - 1) / MIN_CHUNK);

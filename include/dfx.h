@@ -329,7 +329,7 @@ int dfx_layer_impact(const float * x, const float * x_in, int64_t M, int64_t d, 
  * and the split of long caches over the chip (a sequence with more keys is computed all the same).
  * What is out of range is bounded on the device: n_keys is held in 0 .. ld_pages * page_size,
  * rows in 0 .. n_rows, and a page id outside 0 .. n_pages - 1 is no page (its keys are neither
- * written nor seen). */
+ * written nor seen).  A call takes at most 2^23 rows times query heads. */
 typedef struct {
     int32_t type;                /* DFX_TYPE_F16 or DFX_TYPE_F8 */
     int32_t page_size;

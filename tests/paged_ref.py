@@ -207,32 +207,38 @@ def ref_attention(c, b, q, causal, window):
     q = q.astype(np.float64)
     for s, m in enumerate(b.n):
         r0, keys = int(b.rows[s]), min(max(b.keys[s], 0), cap)
-        there = [p for p in range(keys) if b.page_of(s, p, c.n_pages) >= 0]
-        if not there or not m:
+        at = np.array([p for p in range(keys) if b.page_of(s, p, c.n_pages) >= 0], np.int64)
+        if not len(at) or not m:
             continue
+        pos = (keys - m + np.arange(m))[:, None]
+        see = np.ones((m, len(at)), bool)
+        if causal:
+            see &= at <= pos
+            if window:
+                see &= at > pos - window
+        see = np.repeat(see, G, 0)                               # rows of (row, head of the group)
+        some = see.any(1)
         for h in range(c.Hkv):
-            kv = [c.values(b.page_of(s, p, c.n_pages), h, p) for p in there]
-            k, v = np.stack([a for a, _ in kv]), np.stack([a for _, a in kv])
-            at = np.asarray(there)
-            for i in range(m):
-                p = keys - m + i
-                see = np.ones(len(at), bool)
-                if causal:
-                    see &= at <= p
-                    if window:
-                        see &= at > p - window
-                if not see.any():
-                    continue
-                kk, vv = k[see], v[see]
-                for g in range(G):
-                    x = q[r0 + i, h * G + g]
-                    with np.errstate(invalid="ignore", over="ignore"):
-                        sc = kk @ x / np.sqrt(hd)
-                        e = np.exp(sc - np.nanmax(sc)) if not np.isnan(sc).all() else sc
-                        e = e / e.sum()
-                        out[r0 + i, h * G + g] = (e[:, None] * vv).sum(0)
-                        A[r0 + i, h * G + g] = (e[:, None] * np.abs(vv)).sum(0)
-                        E[r0 + i, h * G + g] = (np.abs(kk) @ np.abs(x)).max() / np.sqrt(hd)
+            kv = [c.values(b.page_of(s, int(p), c.n_pages), h, int(p)) for p in at]
+            k, v = np.stack([x for x, _ in kv]), np.stack([x for _, x in kv])
+            x = q[r0:r0 + m, h * G:(h + 1) * G].reshape(m * G, hd)
+            with np.errstate(all="ignore"):
+                # NaN of a hidden key must not reach a row: products only where it is seen
+                sc = np.where(see, x @ np.where(np.isnan(k), 0.0, k).T / np.sqrt(hd), -np.inf)
+                bad = np.isnan(k).any(1)
+                sc = np.where(see & bad, np.nan, sc)
+                top = np.max(np.where(np.isnan(sc), -np.inf, sc), 1, keepdims=True)
+                e = np.where(see, np.exp(sc - np.where(np.isfinite(top), top, 0.0)), 0.0)
+                e = e / e.sum(1, keepdims=True)
+                fine = np.isfinite(v)
+                o, a = e @ np.where(fine, v, 0.0), e @ np.abs(np.where(fine, v, 0.0))
+                for j in np.flatnonzero(~fine.all(1)):           # what is not finite, to the rows that see it
+                    o[see[:, j]] += np.where(fine[j], 0.0, v[j])
+                ee = np.max(np.where(see, np.abs(x) @ np.abs(np.where(np.isnan(k), 0.0, k)).T, 0.0), 1) / np.sqrt(hd)
+            o[~some], a[~some] = 0.0, 0.0
+            out[r0:r0 + m, h * G:(h + 1) * G] = o.reshape(m, G, hd)
+            A[r0:r0 + m, h * G:(h + 1) * G] = a.reshape(m, G, hd)
+            E[r0:r0 + m, h * G:(h + 1) * G] = ee.reshape(m, G)
     return out, A, E
 
 

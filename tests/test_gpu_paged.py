@@ -286,6 +286,50 @@ def test_attention(gpu, case, typ, f32, causal, window):
     assert (got[int(b.rows[-1]):] == 7.0).all()          # rows of no sequence are left
 
 
+# Rows times heads beyond 8192 take 32 queries a workgroup, beyond 32768 128: the same masks, types and ragged
+# batches on those kernels
+WIDE = [([130], [150], 64, 64), ([135, 0, 1], [135, 9, 300], 16, 128), ([70, 33, 40], [340, 33, 64], 32, 64)]
+
+
+@pytest.mark.parametrize("causal,window", [(False, 0), (True, 0), (True, 1), (True, 37)])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("typ", [F8, F16])
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("case", range(len(WIDE)))
+def test_attention_of_many_heads(gpu, case, G, typ, f32, causal, window):
+    n, keys, page, hd = WIDE[case]
+    rng = np.random.default_rng(300 + case)
+    Hkv = 64
+    H = Hkv * G
+    assert sum(n) * H > (32768 if G == 4 else 8192)
+    c = Cache(typ, page, Hkv, hd, sum(-(-k // page) for k in keys) + 2, seed=case)
+    b = Batch(n, keys, page, c.n_pages, seed=case, pad_rows=case % 2)
+    fill_keys(c, b, rng)
+    q = (rng.standard_normal((b.M, H, hd)) * 1.5).astype(np.float32 if f32 else np.float16)
+    got = run_attention(c, b, q, H, causal, window)
+    check_attention(got, c, b, q, causal, window, f32)
+    assert (got[int(b.rows[-1]):] == 7.0).all()
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("Hkv,G,n,keys", [(3, 4, 800, 1400), (8, 5, 900, 1300), (1, 4, 800, 1400)])
+def test_attention_of_long_chunks(gpu, Hkv, G, n, keys, f32):
+    """Many rows over ranges of more than 16 key tiles, with a workspace and without; one KV head's are split over
+    workgroups, where there are enough of them they stay whole and need no workspace."""
+    rng = np.random.default_rng(71)
+    hd, page, H = 64, 64, Hkv * G
+    c = Cache(F8, page, Hkv, hd, -(-keys // page))
+    b = Batch([n], [keys], page, c.n_pages)
+    fill_keys(c, b, rng)
+    q = (rng.standard_normal((n, H, hd)) * 1.5).astype(np.float32 if f32 else np.float16)
+    cd, bd = c.desc(), b.desc()
+    assert L().dfx_paged_attention_ws_bytes(ref(cd), ref(bd), H, F32 if f32 else F16) > 0 or Hkv > 1
+    for causal, window in ((True, 0), (False, 0), (True, 1100)):
+        got = run_attention(c, b, q, H, causal, window)
+        check_attention(got, c, b, q, causal, window, f32)
+        check_attention(run_attention(c, b, q, H, causal, window, ws=False), c, b, q, causal, window, f32)
+
+
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("n,keys", [([1], [5000]), ([1, 1, 2], [3000, 10, 1500]), ([40], [2100])])
 def test_attention_of_long_caches_is_split(gpu, n, keys, f32):
@@ -311,30 +355,32 @@ def test_attention_of_long_caches_is_split(gpu, n, keys, f32):
 
 
 @pytest.mark.parametrize("causal,window", [(False, 0), (True, 0), (True, 20)])
-@pytest.mark.parametrize("S,most", [(63, 2), (64, 30), (65, 3), (150, 40), (70, 150)])
-def test_attention_of_many_sequences(gpu, S, most, causal, window):
+@pytest.mark.parametrize("S,most,Hkv", [(63, 2, 1), (64, 30, 1), (65, 3, 1), (150, 40, 1), (70, 150, 1), (64, 40, 8),
+                                        (70, 40, 8), (64, 60, 16), (75, 60, 16), (5, 90, 40)])
+def test_attention_of_many_sequences(gpu, S, most, Hkv, causal, window):
     """Ragged batches of up to and beyond 64 sequences, empty ones among them, at rows that take each kernel:
     every tile of every sequence is computed once."""
     rng = np.random.default_rng(S + most)
-    Hkv, G, hd, page = 1, 1, 64, 16
+    G, hd, page = 1, 64, 16
     n = [0 if rng.random() < 0.1 else int(rng.integers(most // 2 + 1, most + 1)) for _ in range(S)]
     keys = [m + int(rng.integers(0, 80)) for m in n]
     c = Cache(F8, page, Hkv, hd, sum(-(-k // page) for k in keys))
     b = Batch(n, keys, page, c.n_pages, pad_rows=3)
     fill_keys(c, b, rng)
-    q = (rng.standard_normal((b.M, G, hd)) * 1.5).astype(np.float16)
-    got = run_attention(c, b, q, G, causal, window)
+    q = (rng.standard_normal((b.M, Hkv, hd)) * 1.5).astype(np.float16)
+    got = run_attention(c, b, q, Hkv, causal, window)
     check_attention(got, c, b, q, causal, window, False)
     assert (got[int(b.rows[-1]):] == 7.0).all()
 
 
 @pytest.mark.parametrize("typ", [F8, F16])
-@pytest.mark.parametrize("rows", [1, 30, 100, 200])
-def test_attention_never_sees_hidden_keys(gpu, typ, rows):
+@pytest.mark.parametrize("rows,Hkv", [(1, 1), (30, 1), (100, 1), (200, 1), (90, 64), (200, 90)])
+def test_attention_never_sees_hidden_keys(gpu, typ, rows, Hkv):
     """NaN and infinities in keys and values that some rows see and others do not (later positions, left of
     the window), in the same tile: they reach exactly the rows that see them."""
     rng = np.random.default_rng(40 + rows)
-    Hkv, G, hd, page, keys = 1, 2, 64, 32, 230
+    G, hd, page, keys = 2, 64, 32, 230
+    H, last = Hkv * G, Hkv - 1
     c = Cache(typ, page, Hkv, hd, 9)
     b = Batch([rows], [keys], page, 9)
     fill_keys(c, b, rng)
@@ -342,25 +388,26 @@ def test_attention_never_sees_hidden_keys(gpu, typ, rows):
     for pos, dim, side in ((keys - 3, 5, 1), (keys - 20, 9, 1), (keys - 25, 3, 0), (keys - 60, 1, 1), (100, 60, 1)):
         page_id, t = b.page_of(0, pos, 9), pos % page
         if side:
-            c.v[page_id, 0, t // BLOCK, dim, t % BLOCK] = bad
+            c.v[page_id, last, t // BLOCK, dim, t % BLOCK] = bad
             if not c.f8:
-                c.v[page_id, 0, t // BLOCK, dim + 1, t % BLOCK] = np.inf
-                c.v[page_id, 0, t // BLOCK, dim + 2, t % BLOCK] = -np.inf
+                c.v[page_id, last, t // BLOCK, dim + 1, t % BLOCK] = np.inf
+                c.v[page_id, last, t // BLOCK, dim + 2, t % BLOCK] = -np.inf
         else:
-            c.k[page_id, 0, t, dim] = bad
+            c.k[page_id, last, t, dim] = bad
     c.upload()
     for f32 in (False, True):
-        q = (rng.standard_normal((b.M, G, hd)) * 0.3).astype(np.float32 if f32 else np.float16)
+        q = (rng.standard_normal((b.M, H, hd)) * 0.3).astype(np.float32 if f32 else np.float16)
         for causal, window in ((True, 0), (True, 24), (False, 0)):
-            check_attention(run_attention(c, b, q, G, causal, window), c, b, q, causal, window, f32)
+            check_attention(run_attention(c, b, q, H, causal, window), c, b, q, causal, window, f32)
 
 
+@pytest.mark.parametrize("Hkv", [2, 60, 250])
 @pytest.mark.parametrize("f32", [False, True])
-def test_attention_without_keys_pages_or_rows(gpu, f32):
+def test_attention_without_keys_pages_or_rows(gpu, f32, Hkv):
     """No keys, fewer keys than rows, pages that are none in the middle and throughout: rows without a visible
     key give zeros, the others leave the missing keys out."""
     rng = np.random.default_rng(9)
-    Hkv, G, hd, page = 2, 2, 128, 16
+    G, hd, page = 2, 128, 16
     H = Hkv * G
     c = Cache(F8, page, Hkv, hd, 12)
     pages = np.array([[0, 1, 2, -1], [3, -1, 4, 5], [6, 7, 12, 8], [-1, 1 << 30, -(1 << 31), 12], [9, 10, 11, -7]])
@@ -376,27 +423,29 @@ def test_attention_without_keys_pages_or_rows(gpu, f32):
         check_attention(run_attention(c, b, q, H, causal, 0), c, b, q, causal, 0, f32)
 
 
+@pytest.mark.parametrize("Hkv", [1, 10, 60])
 @pytest.mark.parametrize("rows,keys", [(40, 3), (300, 100), (300, 0), (700, 30)])
-def test_attention_of_more_rows_than_keys(gpu, rows, keys):
+def test_attention_of_more_rows_than_keys(gpu, rows, keys, Hkv):
     """Rows before the first position see nothing under the causal mask: zeros, however many."""
     rng = np.random.default_rng(rows)
-    c = Cache(F8, 16, 1, 64, 12)
+    c = Cache(F8, 16, Hkv, 64, 12)
     b = Batch([rows, 5], [keys, 70], 16, 12)
     fill_keys(c, b, rng)
-    q = rng.standard_normal((b.M, 2, 64)).astype(np.float16)
+    q = rng.standard_normal((b.M, 2 * Hkv, 64)).astype(np.float16)
     for causal in (True, False):
-        check_attention(run_attention(c, b, q, 2, causal, 0), c, b, q, causal, 0, False)
+        check_attention(run_attention(c, b, q, 2 * Hkv, causal, 0), c, b, q, causal, 0, False)
 
 
-def test_attention_of_extreme_queries(gpu):
+@pytest.mark.parametrize("Hkv", [1, 250, 1000])
+def test_attention_of_extreme_queries(gpu, Hkv):
     """f32 queries from 1e-30 to 1e6, zeros, NaN and infinities: a row's range costs no accuracy and its NaN
     stays its own."""
     rng = np.random.default_rng(12)
-    Hkv, G, hd, page = 1, 4, 64, 16
+    G, hd, page = 4, 64, 16
     c = Cache(F16, page, Hkv, hd, 8)
     b = Batch([9], [100], page, 8)
     fill_keys(c, b, rng)
-    q = rng.standard_normal((9, G, hd)).astype(np.float32)
+    q = rng.standard_normal((9, Hkv * G, hd)).astype(np.float32)
     q[1] *= np.float32(1e-30)
     q[2] *= np.float32(1e-5)
     q[3] *= np.float32(300.0)
@@ -404,18 +453,21 @@ def test_attention_of_extreme_queries(gpu):
     q[5, 0, 3] = np.nan
     q[6, 1] *= np.float32(1e-38)
     q[7, 2, :] = 1e6 * np.sign(q[7, 2])
-    check_attention(run_attention(c, b, q, G, True, 0), c, b, q, True, 0, True)
+    check_attention(run_attention(c, b, q, Hkv * G, True, 0), c, b, q, True, 0, True)
     h = np.clip(q, -60000, 60000).astype(np.float16)
-    check_attention(run_attention(c, b, h, G, True, 0), c, b, h, True, 0, False)
+    check_attention(run_attention(c, b, h, Hkv * G, True, 0), c, b, h, True, 0, False)
 
 
+@pytest.mark.parametrize("Hkv", [2, 100])
+@pytest.mark.parametrize("rows", [2, 45, 180])
 @pytest.mark.parametrize("typ", [F8, F16])
-def test_attention_of_extreme_values(gpu, typ):
+def test_attention_of_extreme_values(gpu, typ, rows, Hkv):
     """Values at both ends of the cache's range; an f16 result that overflows is infinite."""
     rng = np.random.default_rng(13)
-    Hkv, hd, page = 2, 64, 16
-    c = Cache(typ, page, Hkv, hd, 10)
-    b = Batch([2, 2], [70, 40], page, 10)
+    hd, page = 64, 16
+    n_pages = 10 if rows == 2 else 40
+    c = Cache(typ, page, Hkv, hd, n_pages)
+    b = Batch([rows, rows], [rows + 68, rows + 38], page, n_pages)
     fill_keys(c, b, rng)
     if c.f8:
         c.scale[..., 1] = np.where(rng.random(c.scale.shape[:3]) < 0.5, 2.0 ** 7, 2.0 ** -15)
@@ -424,7 +476,7 @@ def test_attention_of_extreme_values(gpu, typ):
         c.v[:, 1][np.isfinite(c.v[:, 1])] *= np.float16(2.0 ** -20)
     c.upload()
     for f32 in (True, False):
-        q = rng.standard_normal((4, Hkv, hd)).astype(np.float32 if f32 else np.float16)
+        q = rng.standard_normal((2 * rows, Hkv, hd)).astype(np.float32 if f32 else np.float16)
         check_attention(run_attention(c, b, q, Hkv, False, 0), c, b, q, False, 0, f32)
 
 
@@ -534,6 +586,57 @@ def test_captured_step_follows_the_device_arrays(gpu):
     hip.hipGraphExecDestroy(ex)
     hip.hipGraphDestroy(graph)
     hip.hipStreamDestroy(st)
+
+
+FIRST_CAPTURE = r"""
+import ctypes as C, sys
+import numpy as np
+sys.path[:0] = sys.argv[1:3]
+import dfx
+from paged_ref import Batch, Cache, ref, rope_table
+from test_gpu_paged import fill_keys
+hip, L = C.CDLL("libamdhip64.so"), dfx.lib
+rng = np.random.default_rng(5)
+st = C.c_void_p()
+assert hip.hipStreamCreateWithFlags(C.byref(st), 1) == 0
+# the kernels that take more LDS than a launch has by default: some rows, many rows
+for n, Hkv, G in ((300, 32, 1), (300, 32, 4)):
+    H, hd, page = Hkv * G, 128, 64
+    c = Cache(dfx.TYPE_F16, page, Hkv, hd, 6)
+    b = Batch([n], [n + 20], page, 6)
+    fill_keys(c, b, rng)
+    for typ, nt in ((dfx.TYPE_F16, np.float16), (dfx.TYPE_F32, np.float32)):
+        q = rng.standard_normal((n, H, hd)).astype(nt)
+        dq, do = dfx.Buf.of(q), dfx.Buf.of(np.zeros_like(q))
+        cd, bd = c.desc(), b.desc()
+        graph, ex = C.c_void_p(), C.c_void_p()
+        assert hip.hipStreamBeginCapture(st, 0) == 0                # global capture mode, the first call of its kind
+        rc = L().dfx_paged_attention(ref(cd), ref(bd), dq.ptr, typ, H, 1, 0, do.ptr, None, st)
+        assert hip.hipStreamEndCapture(st, C.byref(graph)) == 0
+        dfx.check(rc, "attention under capture")
+        assert hip.hipGraphInstantiate(C.byref(ex), graph, None, None, 0) == 0
+        de = dfx.Buf.of(np.zeros_like(q))
+        for rep in range(3):
+            do.upload(np.zeros_like(q))
+            dfx.check(L().dfx_paged_attention(ref(cd), ref(bd), dq.ptr, typ, H, 1, 0, de.ptr, None, None))
+            dfx.sync()
+            assert hip.hipGraphLaunch(ex, st) == 0 and hip.hipStreamSynchronize(st) == 0
+            assert np.array_equal(do.download(nt), de.download(nt)) and np.isfinite(do.download(nt)).all()
+print("capture ok")
+"""
+
+
+def test_first_call_under_stream_capture(gpu, tmp_path):
+    """The first call of a process into the kernels whose LDS limit is raised, inside a global-mode capture."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    script = tmp_path / "first.py"
+    script.write_text(FIRST_CAPTURE)
+    r = subprocess.run([sys.executable, str(script), here, os.path.join(os.path.dirname(here), "diffuse-cpp_amd")],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "capture ok" in r.stdout, (r.returncode, r.stdout[-2000:], r.stderr[-2000:])
 
 
 def test_table_of_cells_is_exact(gpu):

@@ -33,7 +33,7 @@ BAD = [(dict(type=dfx.TYPE_Q8_0), {}, -2), (dict(head_dim=96), {}, -2), (dict(pa
        (dict(n_pages=1 << 40), {}, -1), (dict(k=None), {}, -1), (dict(v=None), {}, -1), (dict(scale=None), {}, -1),
        (dict(k=PTR + 8), {}, -1), (dict(v=PTR + 1), {}, -1), (dict(scale=PTR + 4), {}, -1),
        ({}, dict(n_seqs=-1), -1), ({}, dict(n_rows=-1), -1), ({}, dict(max_keys=-1), -1),
-       ({}, dict(n_rows=1 << 30), -1), ({}, dict(rows=None), -1), ({}, dict(n_keys=None), -1),
+       ({}, dict(n_rows=1 << 30), -1), ({}, dict(n_rows=(1 << 20) + 1), -1), ({}, dict(rows=None), -1), ({}, dict(n_keys=None), -1),
        ({}, dict(pages=None), -1), ({}, dict(ld_pages=0), -1)]
 
 
@@ -77,7 +77,7 @@ def test_unsound_scores_are_refused():
              tid=PTR, tlp=PTR, ws=PTR):
         return lp(logits, ld, n_logits, rows, n_rows, V, tokens, n_tok, lpo, ent, n_top, tid, tlp, ws, None)
 
-    for kw in (dict(logits=None), dict(ld=99), dict(V=0), dict(V=1 << 31), dict(n_rows=-1), dict(n_rows=1 << 25),
+    for kw in (dict(logits=None), dict(ld=99), dict(V=0), dict(V=1 << 31), dict(n_rows=-1), dict(n_rows=(1 << 22) + 1),
                dict(n_logits=-1), dict(n_tok=-1), dict(n_top=-1), dict(n_top=65), dict(tokens=None), dict(lpo=None),
                dict(tid=None), dict(tlp=None), dict(ws=None), dict(ws=PTR + 8)):
         assert call(**kw) == -1, kw
