@@ -8,6 +8,8 @@
 #include "dfx_device.h"
 #include "dfx_pages.h"
 
+#include <algorithm>
+
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -368,6 +370,7 @@ static bool aligned(const void * ptr, uintptr_t to) { return ((uintptr_t)ptr & (
 
 // Rows times heads of one call: what a grid of 256-thread workgroups holds in one dimension, halved.
 #define MAX_ROW_HEADS (1 << 23)
+#define MAX_POSITIONS (1 << 30)   // of a sequence: positions a few tiles further are 32-bit integers
 
 // The kernel form of a cache and a batch; a status and message where they are not sound.
 int paged_of(const char * who, const dfx_paged_cache * c, const dfx_paged_batch * b, int n_head, paged_t * out) {
@@ -408,8 +411,7 @@ int paged_of(const char * who, const dfx_paged_cache * c, const dfx_paged_batch 
         dfx_set_error("%s: batch without row offsets, key counts or page ids", who);
         return DFX_ERR_ARG;
     }
-    const int64_t cap = b->ld_pages > (INT32_MAX >> shift) ? (int64_t)(INT32_MAX >> shift) << shift
-                                                           : b->ld_pages << shift;
+    const int64_t cap = std::min<int64_t>(b->ld_pages, MAX_POSITIONS >> shift) << shift;
     *out = {c->k, c->v, c->scale, b->rows, b->n_keys, b->pages, b->ld_pages, (int32_t)c->n_pages, shift, (int32_t)cap,
             c->n_head_kv, b->n_seqs, b->n_rows};
     return DFX_OK;

@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
         have = page_v < 0 ? 0 : pg_clamp(keys - (64 * t + 16 * g), 0, 16);   // tokens of the lane's block that exist
         if constexpr (F8) {
             vs = p.scale[2 * blk + 1];
-            if (page_v < 0) vs = 1.0f;
+            if (have == 0) vs = 1.0f;                               // no page, or not written: anything, NaN too
         }
     };
     bool careful = false;                                           // this wave alone: nothing is shared here
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
             vs[u] = 1.0f;
             if constexpr (F8) {
                 vs[u] = p.scale[2 * blk + 1];
-                if (page_v[u] < 0) vs[u] = 1.0f;
+                if (have[u] == 0) vs[u] = 1.0f;
             }
         }
     };
@@ -956,7 +956,7 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
             have[w] = is ? pg_clamp(keys - 64 * t - 16 * b, 0, 16) : 0;
             if constexpr (F8) {
                 scale[w] = *(const f32x2 *)(p.scale + 2 * blk);
-                if (!is) scale[w] = f32x2{1.0f, 1.0f};
+                if (have[w] == 0) scale[w] = f32x2{1.0f, 1.0f};         // no page, or not written: anything, NaN too
             }
         }
         look_up(t + 1);

@@ -327,8 +327,8 @@ int dfx_layer_impact(const float * x, const float * x_in, int64_t M, int64_t d, 
  * pages[s * ld_pages + p / page_size].  Rows at or behind rows[n_seqs] belong to no sequence and
  * their outputs are left as they were.  max_keys bounds n_keys on the host: it sizes the workspace
  * and the split of long caches over the chip (a sequence with more keys is computed all the same).
- * What is out of range is bounded on the device: n_keys is held in 0 .. ld_pages * page_size,
- * rows in 0 .. n_rows, and a page id outside 0 .. n_pages - 1 is no page (its keys are neither
+ * What is out of range is bounded on the device: n_keys is held in 0 .. ld_pages * page_size (at most
+ * 2^30), rows in 0 .. n_rows, and a page id outside 0 .. n_pages - 1 is no page (its keys are neither
  * written nor seen).  A call takes at most 2^23 rows times query heads. */
 typedef struct {
     int32_t type;                /* DFX_TYPE_F16 or DFX_TYPE_F8 */
@@ -360,7 +360,7 @@ typedef struct {
  * Writing the same positions again (a step over a block of positions that is recomputed) starts
  * with the tokens before them.  A row whose position is negative or not below n_pos is skipped.
  * Two sequences must not write to one page; pages that a sequence only reads may be shared.
- * qkv, tab and q_out start at 16-byte boundaries. */
+ * qkv, tab and q_out start at 16-byte boundaries; q_out does not overlap qkv. */
 int dfx_paged_append(const dfx_paged_cache * cache, const dfx_paged_batch * batch, const float * qkv, int n_head,
                      const float * tab, int64_t n_pos, int q_type, void * q_out, void * stream);
 
@@ -369,7 +369,7 @@ int dfx_paged_append(const dfx_paged_cache * cache, const dfx_paged_batch * batc
  * h / (H / Hkv).  A row at position p sees the keys 0 .. n_keys - 1, or with causal != 0 those up
  * to p, of them with window > 0 (causal only) the last `window`.  A row that sees no key gives
  * zeros; keys that a row does not see never reach it, whatever they hold (NaN included).
- * q, out: [n_rows][H][hd] of `type`, 16-byte aligned: DFX_TYPE_F16 (products of f16 values,
+ * q, out: [n_rows][H][hd] of `type`, 16-byte aligned (out may be q itself): DFX_TYPE_F16 (products of f16 values,
  * f32 sums, probabilities rounded to f16 before P V) or DFX_TYPE_F32 (q and the probabilities
  * split into two f16 terms each: f32 accuracy on the f16 matrix cores).  An f16 `out` is the
  * activation buffer of a dfx_gemm on F16 weights.

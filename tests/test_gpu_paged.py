@@ -401,6 +401,46 @@ def test_attention_never_sees_hidden_keys(gpu, typ, rows, Hkv):
             check_attention(run_attention(c, b, q, H, causal, window), c, b, q, causal, window, f32)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,Hkv", [(1, 1), (90, 64), (200, 90)])
+def test_attention_ignores_scales_of_unwritten_blocks(gpu, rows, Hkv, hd):
+    """Scales behind the last key hold anything, as memory that no append has written does."""
+    rng = np.random.default_rng(60 + rows)
+    G, page, keys = 2, 64, 230
+    c = Cache(F8, page, Hkv, hd, 6)
+    b = Batch([rows], [keys], page, 6)
+    fill_keys(c, b, rng)
+    left = np.array([np.nan, np.inf, -np.inf, 0.0, 1e-40, -3e38, 3.4e38], np.float32)
+    page_id = b.page_of(0, keys, 6)
+    c.scale[page_id, :, 3] = rng.choice(left, c.scale[page_id, :, 3].shape)
+    for other in set(range(6)) - {b.page_of(0, p, 6) for p in range(0, keys, page)}:
+        c.scale[other] = rng.choice(left, c.scale[other].shape)
+    c.upload()
+    for f32 in (False, True):
+        q = rng.standard_normal((b.M, Hkv * G, hd)).astype(np.float32 if f32 else np.float16)
+        for causal in (True, False):
+            check_attention(run_attention(c, b, q, Hkv * G, causal, 0), c, b, q, causal, 0, f32)
+
+
+@pytest.mark.parametrize("rows,keys,Hkv", [(1, 2000, 2), (20, 1300, 2), (90, 230, 64), (200, 230, 90)])
+def test_attention_in_place(gpu, rows, keys, Hkv):
+    """out is q: the bits of the call with two buffers."""
+    rng = np.random.default_rng(80 + rows)
+    H, hd, page = 2 * Hkv, 128, 64
+    c = Cache(F16, page, Hkv, hd, -(-keys // page))
+    b = Batch([rows], [keys], page, c.n_pages)
+    fill_keys(c, b, rng)
+    for f32 in (False, True):
+        q = rng.standard_normal((b.M, H, hd)).astype(np.float32 if f32 else np.float16)
+        want = run_attention(c, b, q, H, True, 0)
+        cd, bd = c.desc(), b.desc()
+        n = L().dfx_paged_attention_ws_bytes(ref(cd), ref(bd), H, F32 if f32 else F16)
+        w, dq = dfx.Buf(n + 16), dfx.Buf.of(q)
+        dfx.check(L().dfx_paged_attention(ref(cd), ref(bd), dq.ptr, F32 if f32 else F16, H, 1, 0, dq.ptr, w.ptr, None))
+        dfx.sync()
+        assert np.array_equal(dq.download(q.dtype, shape=q.shape), want)
+
+
 @pytest.mark.parametrize("Hkv", [2, 60, 250])
 @pytest.mark.parametrize("f32", [False, True])
 def test_attention_without_keys_pages_or_rows(gpu, f32, Hkv):
