@@ -111,9 +111,13 @@ __device__ __forceinline__ f8_choice f8_choose(float amax, bool kept, float old)
 // ---------------------------------------------------------------------------
 // Waves: first the cells, one wave per (RT rows, KV head, side), each taking the blocks whose first
 // row of the call is among its RT rows; then Q, one wave per (rows of one pass, QHEADS heads), whose
-// angles are read once.  RT = 1 where the rows
+// angles are read once (3539 rows of 28 heads: 34.6 us read for each, 26.9 so).  RT = 1 where the rows
 // belong to many sequences (each row enters a block of its own, and one wave per row keeps its chain
 // of dependent loads - places, page, scale, kept cells - alone on it), 16 otherwise.
+// Bound by bytes for prompts, by that chain and the launch for steps.  Measured, heads of 128: 3539 rows of
+// 28 + 4 + 4 heads with f32 Q into E4M3 (120 MB) 26.5 us, 4.5 TB/s (5.1 in a copy); 3583 rows of 32 + 32 +
+// 32 heads into f16 (264 MB) 57.9 us, 4.6 TB/s; one row of 64 sequences of 32 + 32 + 32 heads (4.2 MB) 7.1
+// us; one row 3.8 us.
 #define APPEND_WAVES 4
 #define QHEADS 4
 
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES, 3) k_paged_append(paged_t p
                     for (int k = 0; k < CELL; k++) ow[k] = *(const u32x4 *)(cell + d * WORDS + 4 * k);
 #pragma unroll
                     for (int i = 0; i < WORDS; i++) {
-                        uint32_t keep = 0, kept = 0;                        // bits of tokens outside the new ones, before them
+                        uint32_t keep = 0, kept = 0;                        // bits of tokens not new, and before those
 #pragma unroll
                         for (int e = 0; e < PER; e++) {
                             const int t = i * PER + e;

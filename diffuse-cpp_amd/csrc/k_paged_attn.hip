@@ -153,8 +153,10 @@ template <int T> __device__ __forceinline__ tile_at one_tile(const paged_t & p, 
 // The tiles of the batch in the order of their work, the ones with the most key tiles first (what runs
 // last is short, and neighbours are alike: workgroups go to the parts of the chip in turn).  The weight
 // k of tile t: the largest with more than t tiles of at least that weight, found bit by bit.  Up to 64
-// sequences (a lane each); more: sequence by sequence, each from its end.
-template <int T> __device__ __forceinline__ tile_at wave_tile_by_work(const paged_t & p, int G, int causal, int window, int t) {
+// sequences (a lane each); more: sequence by sequence, each from its end.  (4 causal prompts of 1600 to
+// 3700 tokens: 261 us in the batch's order, 250 in this; interleaved by distance from the end 325.)
+template <int T>
+__device__ __forceinline__ tile_at wave_tile_by_work(const paged_t & p, int G, int causal, int window, int t) {
     const int lane = threadIdx.x & 63;
     if (p.n_seqs > 64 || p.n_seqs == 1) {
         tile_at at = p.n_seqs == 1 ? one_tile<T>(p, G, t) : wave_tile<T>(p, G, t);
@@ -253,9 +255,9 @@ struct attn_t {
 // The four waves' maxima, sums and outputs ([4][T], [4][T], [4][T][HD + 4] in LDS) of a query tile as
 // one: results, or a part of them.
 template <int HD, bool F8, bool F32, int T>
-__device__ __forceinline__ void join_waves(const paged_t & p, const attn_t & a, const tile_at & at, const part_at & pt, int kvh,
-                                           int f0, int f1, const float * so, const float * sm, const float * sl,
-                                           const special_map & map) {
+__device__ __forceinline__ void join_waves(const paged_t & p, const attn_t & a, const tile_at & at, const part_at & pt,
+                                           int kvh, int f0, int f1, const float * so, const float * sm,
+                                           const float * sl, const special_map & map) {
     constexpr int OS = HD + 4;
     const int keys = at.q.keys, p0 = keys - at.q.n;
     const bool special = map.any();
@@ -290,7 +292,8 @@ __device__ __forceinline__ void join_waves(const paged_t & p, const attn_t & a, 
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             v *= inv;
             if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + d) = v;
-            else *(half4 *)((half_t *)a.out + rh * HD + d) = half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+            else *(half4 *)((half_t *)a.out + rh * HD + d) =
+                    half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
         } else {
             const int64_t at_part = (int64_t)blockIdx.y * p.n_rows * a.H + rh;
             *(float4v *)(a.part_o + at_part * HD + d) = v;
@@ -309,10 +312,14 @@ __device__ __forceinline__ void join_waves(const paged_t & p, const attn_t & a, 
 // ---------------------------------------------------------------------------
 // Few rows: 16 queries per workgroup, keys straight from memory
 // ---------------------------------------------------------------------------
-// Bound by the cells' bytes.  Four waves take the 64-key tiles of the workgroup's range in turn and
-// join through LDS at the end.  Lane (i, g) = (lane % 16, lane / 16): query column i; S^T tile u
-// (16 of the 64 keys): row 4b + r is token 4u + r of block b, so the lane's D values (rows 4g + r)
-// over the four tiles are the 16 tokens of block g.
+// Bound by the cells' bytes, and where a workgroup has few tiles by its chain of loads (offsets, page,
+// cells).  Four waves take the 64-key tiles of the workgroup's range in turn and join through LDS at
+// the end.  Lane (i, g) = (lane % 16, lane / 16): query column i; S^T tile u (16 of the 64 keys): row
+// 4b + r is token 4u + r of block b, so the lane's D values (rows 4g + r) over the four tiles are the 16
+// tokens of block g.
+// Measured: 64 sequences of one row, 32 heads of 128, 32469 E4M3 keys in all (266 MB) 70.5 us, 3.8 TB/s
+// (5.1 in a copy); one row of 28 heads over 32701 keys of 4 KV heads (33.5 MB), in 64 parts, 13.5 us and
+// 3.9 of the join.
 #define FEW_T 16
 template <int HD, bool F8, bool F32>
 __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 : 3) k_paged_few(paged_t p, attn_t a) {
@@ -389,8 +396,10 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
     }
 
     // Keys and values take turns in the same registers: the tile's values are loaded when its scores are
-    // taken, the next tile's keys when the values are added.  That leaves room for four workgroups per CU
-    // (F8), whose waves hide each other's loads; the next tile's pages are looked up a tile earlier.
+    // taken, the next tile's keys when the values are added.  That leaves room for three workgroups per CU
+    // (E4M3, 128 dims: 84 registers), whose waves hide each other's loads (the 64 sequences above: 70.5 us;
+    // 78 with keys and values in registers of their own, 141 with both of the next tile on their way); the
+    // next tile's pages are looked up a tile earlier.
     constexpr int CB = F8 ? 1 : 2;
     const int bs = p.page_shift - 4;                                // log2 of a page's blocks
     int page_k = -1, page_v = -1, have = 0;
@@ -453,7 +462,8 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 #pragma unroll
                 for (int w = 0; w < KW; w++) {
                     if constexpr (F8) {
-                        const half8 k0 = f8_half8(cells[u * KW + w].x, cells[u * KW + w].y, ks), k1 = f8_half8(cells[u * KW + w].z, cells[u * KW + w].w, ks);
+                        const u32x4 c = cells[u * KW + w];
+                        const half8 k0 = f8_half8(c.x, c.y, ks), k1 = f8_half8(c.z, c.w, ks);
                         acc = mfma16(k0, qh[2 * w], acc);
                         acc = mfma16(k1, qh[2 * w + 1], acc);
                         if constexpr (F32) {
@@ -579,9 +589,13 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 // ---------------------------------------------------------------------------
 // Some rows: 32 queries per workgroup, keys straight from memory
 // ---------------------------------------------------------------------------
-// k_paged_few with the wider product (32 x 32): four waves take the key steps of the workgroup's range
-// in turn and join through LDS.  A step is KT keys, 64 in 8 bits, 32 in f16 (registers).  Lane (i, h) = (lane % 32, lane / 32), rows of the S^T tiles as
-// in k_paged_many: a lane's 16 D values of tile u are the tokens of block 2u + h in order.
+// k_paged_few with the wider product (32 x 32), which takes half the key reads and matrix operands per
+// query: four waves take the key steps of the workgroup's range in turn and join through LDS.  A step is KT
+// keys, 64 in 8 bits, 32 in f16 (registers).  Lane (i, h) = (lane % 32, lane / 32), rows of the S^T tiles
+// as in k_paged_many: a lane's 16 D values of tile u are the tokens of block 2u + h in order.
+// Bound by latency: two or three workgroups' work per CU.  Measured: 429 f32 rows of 8 sequences, 32 heads of
+// 128, 4525 f16 keys (88 MB) 29.3 us, 3.0 TB/s, the matrix cores busy 13 % of the time; 1414 rows of 6
+// sequences, 8 heads of 64 on 2 KV heads, a window of 512: 11.8 us.
 #define MID_T 32
 template <int HD, bool F8, bool F32>
 __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_mid(paged_t p, attn_t a) {
@@ -594,7 +608,8 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
     extern __shared__ __attribute__((aligned(16))) float so[];              // [4][MID_T][OS]
     __shared__ float sm[4][MID_T], sl[4][MID_T];
     __shared__ special_map map;
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unit_at un = unit_of(blockIdx.x, p.Hkv, a.tiles);
     if (un.kvh >= p.Hkv) return;
     const tile_at at = wave_tile_by_work<MID_T>(p, a.G, a.causal, a.window, un.tile);
@@ -728,7 +743,8 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
 #pragma unroll
                 for (int w = 0; w < KW; w++) {
                     if constexpr (F8) {
-                        const half8 k0 = f8_half8(cells[u][w].x, cells[u][w].y, ks[u]), k1 = f8_half8(cells[u][w].z, cells[u][w].w, ks[u]);
+                        const u32x4 c = cells[u][w];
+                        const half8 k0 = f8_half8(c.x, c.y, ks[u]), k1 = f8_half8(c.z, c.w, ks[u]);
                         s[u] = mfma32(k0, qh[2 * w], s[u]);
                         s[u] = mfma32(k1, qh[2 * w + 1], s[u]);
                         if constexpr (F32) {
@@ -824,7 +840,8 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
                     for (int d = 0; d < DT; d++) {
                         half8 v;
                         if constexpr (F8)
-                            v = j ? f8_half8(cells[u][d * VW].z, cells[u][d * VW].w, vs[u]) : f8_half8(cells[u][d * VW].x, cells[u][d * VW].y, vs[u]);
+                            v = j ? f8_half8(cells[u][d * VW].z, cells[u][d * VW].w, vs[u])
+                                  : f8_half8(cells[u][d * VW].x, cells[u][d * VW].y, vs[u]);
                         else
                             v = __builtin_bit_cast(half8, cells[u][d * VW + j]);
                         o[d] = mfma32(v, ph[2 * u + j], o[d]);
@@ -861,14 +878,21 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
 // ---------------------------------------------------------------------------
 // Many rows: 32 queries per wave, keys through LDS
 // ---------------------------------------------------------------------------
-// Bound by the matrix cores and the exponentials.  Four waves share tiles of 64 keys in LDS, in f16 (so an
-// E4M3 cell is converted once for all of them), two buffers: while a tile is multiplied, the next
-// one's cells are on their way to registers; one barrier per tile.  Lane (i, h) = (lane % 32,
+// Bound by issue: the matrix instructions, the exponentials and the loader's conversions of two waves per
+// SIMD do not overlap fully.  Four waves share tiles of 64 keys in LDS, in f16 (so an E4M3 cell is
+// converted once for all of them), two buffers: while a tile is multiplied, the next one goes from
+// registers to LDS and the one after it is on its way to registers; one barrier per tile.  Lane (i, h) = (lane % 32,
 // lane / 32): query column i; S^T tile u (32 of the 64 keys): row 8a + 4b + r is token 4a + r of block
 // 2u + b, so the lane's 16 D values are the 16 tokens of block 2u + h in order.
 // LDS: K by 8-dim chunks, [HD / 8][64 tokens in S^T row order][16 B]; V by halves of blocks,
 // [4 blocks][2][HD][16 B]: every operand read is 64 lanes of consecutive 16 bytes per half wave.
 // The running maximum is let lag (by up to 2^8): sums are rescaled only where it moves further.
+// Measured: 4 causal prompts, 9716 rows of 28 heads on 4 E4M3 KV heads of 128, 188.6 GFLOP: 239 us, 789
+// TFLOP/s (a library's square f16 product of 8192: 1212), the matrix cores busy 37 % of the time.  Of 250 us
+// in an earlier state the loads took 28, the stores to LDS and their conversions 33, the exponentials 11
+// (each left out in turn).  Other forms, beside 250: 64 queries a wave (two columns of tiles) 405, as the
+// accumulators no longer fit the vector registers; 256 queries a workgroup 254; scores of the next tile
+// taken before this one's values are added 258-275.
 template <int HD> struct many_lds {
     static constexpr int KS = 64 * 16 + 16;             // bytes per key chunk (the rest of a bank row: writes spread)
     static constexpr int VS = HD * 16 + 64;             // bytes per half block of values
@@ -892,7 +916,8 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     int * flags = (int *)(lds + 2 * (lds_t::K + lds_t::V));      // [2][4], the mark of a careful pass
     special_map & map = *(special_map *)(flags + 12);
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unit_at un = unit_of(blockIdx.x, p.Hkv, a.tiles);
     if (un.kvh >= p.Hkv) return;
     const tile_at at = wave_tile_by_work<T>(p, a.G, a.causal, a.window, un.tile);
@@ -1042,8 +1067,8 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
         return *(const half8 *)(lds + buf * (lds_t::K + lds_t::V) + (2 * c + h) * lds_t::KS + (32 * u + i) * 16);
     };
     auto read_v = [&](int buf, int d, int g) __attribute__((always_inline)) {   // (u, half of the block) = (g / 2, g % 2)
-        return *(const half8 *)(lds + buf * (lds_t::K + lds_t::V) + lds_t::K + (2 * (2 * (g >> 1) + h) + (g & 1)) * lds_t::VS +
-                                (32 * d + i) * 16);
+        return *(const half8 *)(lds + buf * (lds_t::K + lds_t::V) + lds_t::K +
+                                (2 * (2 * (g >> 1) + h) + (g & 1)) * lds_t::VS + (32 * d + i) * 16);
     };
     // operands read ahead of their products: fewer where f32 results and f16 cells need the registers
     constexpr int KH = QS / (F32 && !F8 ? 4 : 2), VH = DT / (F32 && !F8 && DT == 4 ? 4 : 2);
@@ -1052,7 +1077,8 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
     half8 ph[4], pl[F32 ? 4 : 1];
     auto mask = [&](float16v (&s)[2], int buf, int t) __attribute__((always_inline)) {
         const int4 there = *(const int4 *)(flags + 4 * buf);
-        if (64 * t >= last.lo && 64 * t + 63 <= first.hi && min(min(there.x, there.y), min(there.z, there.w)) == 16) return;
+        const bool whole = min(min(there.x, there.y), min(there.z, there.w)) == 16;
+        if (whole && 64 * t >= last.lo && 64 * t + 63 <= first.hi) return;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int k0 = 64 * t + 32 * u + 16 * h;
@@ -1218,7 +1244,8 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
             const int dim = 32 * d + 8 * b + 4 * h;
             const float4v v = {o[d][4 * b] * mul, o[d][4 * b + 1] * mul, o[d][4 * b + 2] * mul, o[d][4 * b + 3] * mul};
             if constexpr (F32) *(float4v *)((float *)a.out + rh * HD + dim) = v;
-            else *(half4 *)((half_t *)a.out + rh * HD + dim) = half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
+            else *(half4 *)((half_t *)a.out + rh * HD + dim) =
+                    half4{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
         }
 }
 
@@ -1228,7 +1255,8 @@ __global__ void __launch_bounds__(64 * MANY_WAVES, 2) k_paged_many(paged_t p, at
 // o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  W waves per (row, head): half a wave reads a part's
 // sums, HD / 32 dims a lane, so W waves take 2 W parts at a time, all that there may be (ALL of them per
 // half wave) before any is known to be needed: one round of loads.  The sums are added in a fixed
-// order: the same bits on every run.
+// order: the same bits on every run.  28 rows and heads of 64 parts (0.9 MB): 3.9 us, a launch and two
+// dependent loads.
 template <int HD, bool F32, int W, int ALL>
 __global__ void __launch_bounds__(256) k_paged_join(paged_t p, attn_t a) {
     constexpr int DL = HD / 32;                                 // dims per lane
@@ -1411,7 +1439,8 @@ extern "C" int dfx_paged_attention(const dfx_paged_cache * cache, const dfx_page
     }
     const int hd = cache->head_dim;
     const attn_plan pl = plan_of(p, n_head, batch->max_keys, window, ws != nullptr);
-    attn_t a = {q, out, (float *)ws, nullptr, nullptr, n_head, n_head / p.Hkv, causal ? 1 : 0, window, pl.chunk, pl.parts, pl.tiles};
+    attn_t a = {q,      out,      (float *)ws, nullptr, nullptr, n_head, n_head / p.Hkv, causal ? 1 : 0, window, pl.chunk,
+                pl.parts, pl.tiles};
     a.part_ml = a.part_o + (size_t)pl.parts * p.n_rows * n_head * hd;
     a.n_parts = (int32_t *)(a.part_ml + (size_t)pl.parts * p.n_rows * n_head * 2);
     hipStream_t st = (hipStream_t)stream;
