@@ -328,7 +328,9 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
     constexpr int KW = F8 ? HD / 64 : HD / 32;  // 16-byte loads of a lane per S tile
     constexpr int VW = F8 ? 1 : 2;              // 16-byte loads of a lane per O tile
     constexpr int OS = HD + 4;                  // LDS floats per query
-    __shared__ float so[4][FEW_T][OS];
+    constexpr bool QL = F32 && F8;              // Q's terms in LDS, read in every turn
+    __shared__ __attribute__((aligned(16))) float so[4][FEW_T][OS];         // Q's terms, then the waves' sums
+    static_assert(sizeof(so) >= KS * 2 * 64 * sizeof(half8), "room for Q's terms");
     __shared__ float sm[4][FEW_T], sl[4][FEW_T];
     __shared__ special_map map;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -347,7 +349,8 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
     const seen_t me = pg_seen(p0 + f / a.G, keys, a.causal, a.window);
 
     // ---- Q: step s holds dims in the order in which the lane's key loads bring them
-    half8 qh[KS], ql[KS];
+    half8 qh[QL ? 1 : KS], ql[QL ? 1 : KS];
+    half8 * const qs = (half8 *)&so[0][0][0] + lane;    // step s: the terms at 128 s and 128 s + 64
     float sc = LOG2E_F / sqrtf((float)HD);
     {
         const int64_t qo = ((int64_t)row * a.H + head) * HD;
@@ -369,14 +372,23 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
             const int ex = q_exponent(quad_max(amax));
             sc = ldexpf(sc, ex);
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++) {
+                half8 th, tl;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     half_t hi, lo;
                     split16(ldexpf(x[s][k], -ex), hi, lo);
-                    qh[s][k] = hi;
-                    ql[s][k] = lo;
+                    th[k] = hi;
+                    tl[k] = lo;
                 }
+                if constexpr (!QL) {
+                    qh[s] = th;
+                    ql[s] = tl;
+                } else if (s % 4 == wv) {                           // the four waves' queries are the same
+                    qs[128 * s] = th;
+                    qs[128 * s + 64] = tl;
+                }
+            }
         } else {
 #pragma unroll
             for (int s = 0; s < KS; s++) qh[s] = *(const half8 *)((const half_t *)a.q + qo + dim(s));
@@ -389,11 +401,12 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
     float4v o[DT];
 
     // Q is waited for here, not inside the loop (where the wait would be for the next tile's loads)
+    if constexpr (!QL)
 #pragma unroll
-    for (int c = 0; c < KS; c++) {
-        asm volatile("" : "+v"(qh[c]));
-        if constexpr (F32) asm volatile("" : "+v"(ql[c]));
-    }
+        for (int c = 0; c < KS; c++) {
+            asm volatile("" : "+v"(qh[c]));
+            if constexpr (F32) asm volatile("" : "+v"(ql[c]));
+        }
 
     // Keys and values take turns in the same registers: the tile's values are loaded when its scores are
     // taken, the next tile's keys when the values are added.  That leaves room for three workgroups per CU
@@ -455,6 +468,13 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
             }
         }
         for (int t = pt.t0 + wv; t < pt.t1; t += 4) {
+            if constexpr (QL) asm volatile("" ::: "memory");       // not kept in registers from turn to turn
+            half8 qa[KS], qb[KS];
+#pragma unroll
+            for (int c = 0; c < KS; c++) {
+                qa[c] = QL ? qs[128 * c] : qh[QL ? 0 : c];
+                if constexpr (F32) qb[c] = QL ? qs[128 * c + 64] : ql[QL ? 0 : c];
+            }
             float s[16];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
@@ -464,16 +484,16 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
                     if constexpr (F8) {
                         const u32x4 c = cells[u * KW + w];
                         const half8 k0 = f8_half8(c.x, c.y, ks), k1 = f8_half8(c.z, c.w, ks);
-                        acc = mfma16(k0, qh[2 * w], acc);
-                        acc = mfma16(k1, qh[2 * w + 1], acc);
+                        acc = mfma16(k0, qa[2 * w], acc);
+                        acc = mfma16(k1, qa[2 * w + 1], acc);
                         if constexpr (F32) {
-                            acc = mfma16(k0, ql[2 * w], acc);
-                            acc = mfma16(k1, ql[2 * w + 1], acc);
+                            acc = mfma16(k0, qb[2 * w], acc);
+                            acc = mfma16(k1, qb[2 * w + 1], acc);
                         }
                     } else {
                         const half8 k0 = __builtin_bit_cast(half8, cells[u * KW + w]);
-                        acc = mfma16(k0, qh[w], acc);
-                        if constexpr (F32) acc = mfma16(k0, ql[w], acc);
+                        acc = mfma16(k0, qa[w], acc);
+                        if constexpr (F32) acc = mfma16(k0, qb[w], acc);
                     }
                 }
 #pragma unroll
@@ -576,6 +596,7 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 
     // ---- the four waves' results
     l = quad_sum(l);
+    if constexpr (QL) __syncthreads();                              // Q has been read
     if (g == 0) {
         sm[wv][i] = m;
         sl[wv][i] = l;
@@ -598,14 +619,15 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 // sequences, 8 heads of 64 on 2 KV heads, a window of 512: 11.8 us.
 #define MID_T 32
 template <int HD, bool F8, bool F32>
-__global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_mid(paged_t p, attn_t a) {
+__global__ void __launch_bounds__(256, 2) k_paged_mid(paged_t p, attn_t a) {
     constexpr int U = F8 ? 2 : 1, KT = 32 * U;
     constexpr int QS = HD / 16, DT = HD / 32;
     constexpr int KW = F8 ? HD / 32 : HD / 16;  // 16-byte loads of a lane per S tile
     constexpr int VW = F8 ? 1 : 2;              // 16-byte loads of a lane per O tile and S tile
     constexpr int CB = F8 ? 1 : 2;
     constexpr int OS = HD + 4;                  // LDS floats per query
-    extern __shared__ __attribute__((aligned(16))) float so[];              // [4][MID_T][OS]
+    constexpr bool QL = F32 && F8;              // Q's terms in LDS, read in every turn
+    extern __shared__ __attribute__((aligned(16))) float so[];              // Q's terms, then [4][MID_T][OS]
     __shared__ float sm[4][MID_T], sl[4][MID_T];
     __shared__ special_map map;
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
@@ -624,7 +646,8 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
     const seen_t me = pg_seen(p0 + f / a.G, keys, a.causal, a.window);
 
     // ---- Q: step c holds dims in the order in which the lane's key loads bring them
-    half8 qh[QS], ql[F32 ? QS : 1];
+    half8 qh[QL ? 1 : QS], ql[F32 && !QL ? QS : 1];
+    half8 * const qs = (half8 *)so + lane;      // step c: the terms at 128 c and 128 c + 64
     float sc = LOG2E_F / sqrtf((float)HD);
     {
         const int64_t qo = ((int64_t)row * a.H + head) * HD;
@@ -646,14 +669,23 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
             const int ex = q_exponent(half_max(amax));
             sc = ldexpf(sc, ex);
 #pragma unroll
-            for (int c = 0; c < QS; c++)
+            for (int c = 0; c < QS; c++) {
+                half8 th, tl;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     half_t hi, lo;
                     split16(ldexpf(x[c][k], -ex), hi, lo);
-                    qh[c][k] = hi;
-                    ql[c][k] = lo;
+                    th[k] = hi;
+                    tl[k] = lo;
                 }
+                if constexpr (!QL) {
+                    qh[c] = th;
+                    ql[c] = tl;
+                } else if (c % 4 == wv) {                           // the four waves' queries are the same
+                    qs[128 * c] = th;
+                    qs[128 * c + 64] = tl;
+                }
+            }
         } else {
 #pragma unroll
             for (int c = 0; c < QS; c++) qh[c] = *(const half8 *)((const half_t *)a.q + qo + dim(c));
@@ -661,11 +693,12 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
     }
     if (threadIdx.x < MAP_BITS / 32) map.w[threadIdx.x] = 0;
     __syncthreads();
+    if constexpr (!QL)
 #pragma unroll
-    for (int c = 0; c < QS; c++) {                                  // waited for here, as in k_paged_few
-        asm volatile("" : "+v"(qh[c]));
-        if constexpr (F32) asm volatile("" : "+v"(ql[c]));
-    }
+        for (int c = 0; c < QS; c++) {                              // waited for here, as in k_paged_few
+            asm volatile("" : "+v"(qh[c]));
+            if constexpr (F32) asm volatile("" : "+v"(ql[c]));
+        }
 
     const int bs = p.page_shift - 4;
     const int s0 = pt.t0 * (64 / KT), s1 = pt.t1 * (64 / KT);       // key steps
@@ -735,27 +768,33 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
             load_k(s0 + wv);
         }
         for (int st = s0 + wv; st < s1; st += 4) {
+            if constexpr (QL) asm volatile("" ::: "memory");       // not kept in registers from turn to turn
             float16v s[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
+            for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < KW; w++) {
+            for (int c = 0; c < QS; c++) {
+                half8 qa, qb;
+                if constexpr (QL) {
+                    qa = qs[128 * c];
+                    qb = qs[128 * c + 64];
+                } else {
+                    qa = qh[c];
+                    if constexpr (F32) qb = ql[c];
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    half8 k;
                     if constexpr (F8) {
-                        const u32x4 c = cells[u][w];
-                        const half8 k0 = f8_half8(c.x, c.y, ks[u]), k1 = f8_half8(c.z, c.w, ks[u]);
-                        s[u] = mfma32(k0, qh[2 * w], s[u]);
-                        s[u] = mfma32(k1, qh[2 * w + 1], s[u]);
-                        if constexpr (F32) {
-                            s[u] = mfma32(k0, ql[2 * w], s[u]);
-                            s[u] = mfma32(k1, ql[2 * w + 1], s[u]);
-                        }
+                        const u32x4 w = cells[u][c / 2];
+                        k = c % 2 ? f8_half8(w.z, w.w, ks[u]) : f8_half8(w.x, w.y, ks[u]);
                     } else {
-                        const half8 k0 = __builtin_bit_cast(half8, cells[u][w]);
-                        s[u] = mfma32(k0, qh[w], s[u]);
-                        if constexpr (F32) s[u] = mfma32(k0, ql[w], s[u]);
+                        k = __builtin_bit_cast(half8, cells[u][c]);
                     }
+                    s[u] = mfma32(k, qa, s[u]);
+                    if constexpr (F32) s[u] = mfma32(k, qb, s[u]);
                 }
             }
             load_v(st);
@@ -861,6 +900,7 @@ __global__ void __launch_bounds__(256, HD == 128 && F8 && F32 ? 1 : 2) k_paged_m
 
     // ---- the four waves' results
     l = half_sum(l);
+    if constexpr (QL) __syncthreads();                              // Q has been read
     if (h == 0) {
         sm[wv][i] = m;
         sl[wv][i] = l;
@@ -1389,6 +1429,7 @@ static int attn_launch(const paged_t & p, const attn_t & a, const attn_plan & pl
     else if (pl.T == MID_T) {
         static std::atomic<uint64_t> set;
         constexpr int bytes = 4 * MID_T * (HD + 4) * (int)sizeof(float);
+        static_assert(bytes >= (HD / 16) * 2 * 64 * (int)sizeof(half8), "room for Q's terms");
         rc = many_lds_limit((const void *)k_paged_mid<HD, F8, F32>, bytes, set);
         if (rc == DFX_OK) hipLaunchKernelGGL((k_paged_mid<HD, F8, F32>), grid, dim3(256), bytes, st, p, a);
     }
