@@ -319,7 +319,9 @@ __device__ __forceinline__ void join_waves(const paged_t & p, const attn_t & a, 
 // tokens of block g.
 // Measured: 64 sequences of one row, 32 heads of 128, 32469 E4M3 keys in all (266 MB) 70.5 us, 3.8 TB/s
 // (5.1 in a copy); one row of 28 heads over 32701 keys of 4 KV heads (33.5 MB), in 64 parts, 13.5 us and
-// 3.9 of the join.
+// 3.9 of the join.  64 equal ranges of 1001 keys: 97 us from E4M3 cells (5.4 TB/s), 179 from f16 (5.9).
+// f32 queries of E4M3 caches are kept in LDS: in registers the third workgroup per CU spilled, and those 64
+// ranges took 128 us, 102 so.  (f16 cells leave room for two workgroups either way: no difference.)
 #define FEW_T 16
 template <int HD, bool F8, bool F32>
 __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 : 3) k_paged_few(paged_t p, attn_t a) {
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 
     // Keys and values take turns in the same registers: the tile's values are loaded when its scores are
     // taken, the next tile's keys when the values are added.  That leaves room for three workgroups per CU
-    // (E4M3, 128 dims: 84 registers), whose waves hide each other's loads (the 64 sequences above: 70.5 us;
+    // (E4M3, 128 dims: 168 registers), whose waves hide each other's loads (the 64 sequences above: 70.5 us;
     // 78 with keys and values in registers of their own, 141 with both of the next tile on their way); the
     // next tile's pages are looked up a tile earlier.
     constexpr int CB = F8 ? 1 : 2;
@@ -614,7 +616,9 @@ __global__ void __launch_bounds__(256, !F8 ? (HD == 64 ? 3 : 2) : HD == 64 ? 4 :
 // query: four waves take the key steps of the workgroup's range in turn and join through LDS.  A step is KT
 // keys, 64 in 8 bits, 32 in f16 (registers).  Lane (i, h) = (lane % 32, lane / 32), rows of the S^T tiles
 // as in k_paged_many: a lane's 16 D values of tile u are the tokens of block 2u + h in order.
-// Bound by latency: two or three workgroups' work per CU.  Measured: 429 f32 rows of 8 sequences, 32 heads of
+// Bound by latency: two or three workgroups' work per CU.  f32 queries of E4M3 caches are in LDS: registers
+// for two workgroups per CU instead of one (4 x 128 rows of 32 heads over 828 keys 44.3 us, 30.3 so; with
+// f16 cells two fit either way, and three, with Q in LDS, spill: 29.3 us to 36.5).  Measured: 429 f32 rows of 8 sequences, 32 heads of
 // 128, 4525 f16 keys (88 MB) 29.3 us, 3.0 TB/s, the matrix cores busy 13 % of the time; 1414 rows of 6
 // sequences, 8 heads of 64 on 2 KV heads, a window of 512: 11.8 us.
 #define MID_T 32
