@@ -1389,13 +1389,20 @@ static attn_plan plan_of(const paged_t & p, int H, int64_t max_keys, int window,
     r.T = queries <= 16 * seqs || all <= 512 * 16 ? FEW_T : queries <= 32 * seqs || all <= 1024 * 32 ? MID_T : MANY_T;
     r.tiles = (int)(queries / r.T + seqs);
     const int64_t units = (int64_t)p.Hkv * std::max<int64_t>(seqs, queries / r.T);
-    // 32 and 128 queries come in more than 256 workgroups (8192 / 32, 32768 / 128): their ranges stay whole
-    const int64_t want = r.T == FEW_T ? std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, 512 / units)) : 1;
+    // Parts of kt key tiles: as many as make 512 workgroups, and where the parts still have 16 tiles up to 2048,
+    // as a batch's ranges are seldom equal (32 sequences of 17 to 4000 keys, 32 heads: 64.5 us whole, 55 in two
+    // parts; 96 such of 4 KV heads 33.6 / 27.6 in three; 16 of 2000 61.3 / 57.2; 96 equal ones of 2000, 4 KV
+    // heads, lose: 42.2 / 45.8; 64 of 32 heads, 2048 workgroups, stay whole: 69.8 / 76.7).  32 and 128 queries
+    // come in more than 256 workgroups (8192 / 32, 32768 / 128): their ranges stay whole.
+    const auto want = [&](int64_t kt) {
+        const int64_t n = std::max<int64_t>(512 / units, std::min<int64_t>(kt / WHOLE, 2048 / units));
+        return r.T == FEW_T ? std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, n)) : 1;
+    };
     // key tiles that a query tile can see
     int64_t kt = (std::min<int64_t>(std::max<int64_t>(max_keys, 1), p.cap) + 63) / 64;
-    r.most = kt <= WHOLE ? 1 : (int)std::min<int64_t>(want, (kt + MIN_CHUNK - 1) / MIN_CHUNK);
+    r.most = kt <= WHOLE ? 1 : (int)std::min<int64_t>(want(kt), (kt + MIN_CHUNK - 1) / MIN_CHUNK);
     if (window > 0) kt = std::min<int64_t>(kt, ((int64_t)window + r.T / G + 63) / 64 + 1);
-    r.chunk = (int)std::max<int64_t>(MIN_CHUNK, (kt + want - 1) / want);
+    r.chunk = (int)std::max<int64_t>(MIN_CHUNK, (kt + want(kt) - 1) / want(kt));
     r.parts = split && kt > WHOLE ? (int)((kt + r.chunk - 1) / r.chunk) : 1;
     return r;
 }

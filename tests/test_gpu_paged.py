@@ -373,6 +373,28 @@ def test_attention_of_many_sequences(gpu, S, most, Hkv, causal, window):
     assert (got[int(b.rows[-1]):] == 7.0).all()
 
 
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("S,Hkv,window", [(40, 16, 0), (40, 16, 1100), (70, 8, 0)])
+def test_attention_of_uneven_sequences_is_split(gpu, S, Hkv, window, f32):
+    """Few long sequences among many short ones: long ranges in parts beside whole ones, some without keys."""
+    rng = np.random.default_rng(90 + S)
+    G, hd, page = 2, 64, 64
+    n = [int(rng.integers(0, 3)) for _ in range(S)]
+    keys = [int(rng.integers(0, 70)) for _ in range(S)]
+    for s, k in ((0, 2300), (S // 2, 1500), (S - 1, 1030)):
+        n[s], keys[s] = 1 + s % 2, k
+    c = Cache(F8, page, Hkv, hd, sum(-(-k // page) for k in keys) + 1)
+    b = Batch(n, keys, page, c.n_pages, seed=S, pad_rows=2)
+    fill_keys(c, b, rng)
+    H = Hkv * G
+    q = (rng.standard_normal((b.M, H, hd)) * 1.5).astype(np.float32 if f32 else np.float16)
+    cd, bd = c.desc(), b.desc()
+    assert L().dfx_paged_attention_ws_bytes(ref(cd), ref(bd), H, F32 if f32 else F16) > 0
+    got = run_attention(c, b, q, H, True, window)
+    check_attention(got, c, b, q, True, window, f32)
+    assert (got[int(b.rows[-1]):] == 7.0).all()
+
+
 @pytest.mark.parametrize("typ", [F8, F16])
 @pytest.mark.parametrize("rows,Hkv", [(1, 1), (30, 1), (100, 1), (200, 1), (90, 64), (200, 90)])
 def test_attention_never_sees_hidden_keys(gpu, typ, rows, Hkv):
